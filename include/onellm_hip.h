@@ -274,6 +274,58 @@ int onellm_topk_sample(const int* topk_id, const float* topk_val, int* output_id
                        unsigned char* is_finished, int B, int K, unsigned long long seed, int end_id,
                        int vocab_size, onellm_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Serving from a paged key-value cache.  No counterpart in the reference, whose cache reserves S rows for every
+ * sequence (src/kernels/decoder_masked_attn.cu:136-327) and whose prompt attention is a chain of GEMM-sized launches
+ * over padded buffers (src/layers/attention/context_attention.cpp:117-134).
+ *
+ * k_pages, v_pages [num_layers, num_pages, Hkv, page_size, D]; slab `layer` is used.  page_size is a power of two of 16 or more.
+ * block_table device int32[B, max_pages]: entry p of row b is the page that holds rows p * page_size .. of sequence b.  Pages
+ * may be shared between sequences as long as no call writes a shared one.  An entry outside [0, num_pages) - and any
+ * row past max_pages * page_size - is "no page": its rows are neither read nor written and take no part in any sum.
+ * D <= 256 and a whole number of 16-byte pieces (a multiple of 8 in fp16, of 4 in fp32); all buffers 16-byte aligned;
+ * token strides (in elements) whole 16-byte pieces; B <= 65535, Hq <= 4096, max_pages * page_size < 2^30.  Anything else is
+ * ONELLM_EUNSUPPORTED.
+ * Packed tokens: sequence b owns tokens cu_tokens[b] .. cu_tokens[b + 1] - 1 (device int32[B + 1], ascending, inside
+ * [0, token_num]; sequences may be empty) and had history_length[b] rows before them (device int32[B]); token i of a
+ * sequence sits at position history_length[b] + i.  Tokens of no sequence, and those of a sequence with a negative history, are left
+ * as they are.
+ * ---------------------------------------------------------------------------------------------- */
+
+/*
+ * Packed tokens into the cache: QKV bias, rotary positions, k and v rows to their pages, q to q_out.
+ *   qkv [token_num, Hq + 2 Hkv, D]; qkv_bias as in onellm_decode_attn (may be NULL);
+ *   q_out: token i's heads at q_out + i * q_stride elements, [Hq, D] each.  q_out may be qkv with q_stride = (Hq + 2 Hkv) * D
+ *   (q is rotated in place); any other overlap is ONELLM_EINVAL.
+ * Rotation as in onellm_decode_attn (adjacent pairs, rotary_dim even); the angle is reduced in 64 bits, so a far position is
+ * rotated as exactly as a near one.
+ */
+int onellm_paged_qkv_store(int dtype, void* q_out, long q_stride, void* k_pages, void* v_pages,
+                           const void* qkv, const void* qkv_bias,
+                           const int* cu_tokens, const int* history_length, const int* block_table,
+                           int B, int token_num, int Hq, int Hkv, int D,
+                           int page_size, int num_pages, int max_pages, int layer, int num_layers,
+                           int rotary_dim, float rope_base, onellm_stream_t stream);
+
+/*
+ * Causal attention of packed tokens over the paged cache, which holds their own rows already (onellm_paged_qkv_store):
+ *   out[i] = sum_j softmax_j(q[i] . k[j] / sqrt(D)) v[j]   over the rows j <= history_length[b] + i that have a page
+ * for all Hq heads, kv head h / (Hq / Hkv).  A token that sees no row gets zeros.  q, out: token i at q + i * q_stride,
+ * out + i * out_stride elements; out may be q.
+ *   max_rows   upper bound of every sequence's history + tokens; where few tokens meet many rows it sizes the cut of the
+ *              rows into pieces (a longer sequence is still attended in full, slower)
+ *   workspace  onellm_paged_prompt_attn_workspace_bytes() bytes, 256-byte aligned, contents irrelevant; calls that share one
+ *              must not overlap
+ * Scores, statistics and sums are fp32; fp16 weights enter their product rounded to fp16.
+ */
+int onellm_paged_prompt_attn(int dtype, const void* q, long q_stride, const void* k_pages, const void* v_pages,
+                             void* out, long out_stride,
+                             const int* cu_tokens, const int* history_length, const int* block_table,
+                             int B, int token_num, int Hq, int Hkv, int D,
+                             int page_size, int num_pages, int max_pages, int layer, int num_layers,
+                             int max_rows, void* workspace, size_t workspace_bytes, onellm_stream_t stream);
+size_t onellm_paged_prompt_attn_workspace_bytes(int B, int token_num, int Hq, int Hkv, int D, int max_rows);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,7 @@ TOPK_PATH_ONE_LAUNCH, TOPK_PATH_TWO_LAUNCHES, TOPK_PATH_NO_COUNTER_SET = 1, 2, 3
 
 # every symbol include/onellm_hip.h declares: name -> (restype, argtypes)
 _vp, _ci, _cf, _cu, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_uint, ctypes.c_size_t
+_cl = ctypes.c_long
 SYMBOLS = {
     "onellm_hip_version": (_ci, []),
     "onellm_error_string": (ctypes.c_char_p, [_ci]),
@@ -45,6 +46,9 @@ SYMBOLS = {
                                              _cf, _vp]),
     "onellm_silu_and_mul": (_ci, [_ci, _vp, _vp, _ci, _ci, _vp]),
     "onellm_topk_sample": (_ci, [_vp, _vp, _vp, _vp, _vp, _ci, _ci, ctypes.c_ulonglong, _ci, _ci, _vp]),
+    "onellm_paged_qkv_store": (_ci, [_ci, _vp, _cl, _vp, _vp, _vp, _vp, _vp, _vp, _vp] + [_ci] * 11 + [_cf, _vp]),
+    "onellm_paged_prompt_attn": (_ci, [_ci, _vp, _cl, _vp, _vp, _vp, _cl, _vp, _vp, _vp] + [_ci] * 11 + [_vp, _sz, _vp]),
+    "onellm_paged_prompt_attn_workspace_bytes": (_sz, [_ci, _ci, _ci, _ci, _ci, _ci]),
 }
 
 _lib = None
@@ -245,6 +249,94 @@ def topk_sample(topk_id, topk_val, output_id, seqlen, is_finished, seed, end_id,
     _check(lib().onellm_topk_sample(_ptr(topk_id), _ptr(topk_val), _ptr(output_id), _ptr(seqlen), _ptr(is_finished), B, K,
                                     int(seed), end_id, vocab_size, _stream()), "onellm_topk_sample")
     return output_id
+
+
+# ---------------------------------------------------------------- serving from a paged key-value cache
+
+def _same_device(*tensors):
+    """The calls below launch on the current device's stream: everything they are handed has to live there."""
+    import torch
+    here = torch.device("cuda", torch.cuda.current_device())
+    for t in tensors:
+        if t is not None and t.device != here:
+            raise ValueError(f"tensor on {t.device}, but the current device is {here}")
+
+
+def _int32(*tensors):
+    import torch
+    for t in tensors:
+        if t is not None and t.dtype != torch.int32:
+            raise TypeError(f"int32 tensor expected, not {t.dtype}")
+
+
+def _rows(t, what):
+    """(pointer, token stride) of a [tokens, heads, D] tensor whose tokens may be a stride apart"""
+    if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
+        raise ValueError(f"{what}: [tokens, heads, D] with contiguous heads expected")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * t.shape[2])
+
+
+def _pages(k_pages, v_pages, block_table, dtype):
+    if k_pages.dim() != 5 or k_pages.shape != v_pages.shape or k_pages.dtype != dtype or v_pages.dtype != dtype:
+        raise ValueError("k_pages, v_pages: [layers, pages, Hkv, page_size, D] of the activations' type expected")
+    if block_table.dim() != 2:
+        raise ValueError("block_table: [B, max_pages] expected")
+    return k_pages.shape
+
+
+def _packed(cu_tokens, history_length, block_table):
+    B = block_table.shape[0]
+    if cu_tokens.numel() != B + 1 or history_length.numel() != B:
+        raise ValueError("cu_tokens [B + 1], history_length [B] and block_table [B, max_pages] expected")
+    return B
+
+
+def paged_qkv_store(q_out, k_pages, v_pages, qkv, bias, cu_tokens, history_length, block_table, rotary_dim, rope_base, layer=0):
+    """qkv [tokens, Hq+2Hkv, D]; q_out [tokens, Hq, D] (may be qkv[:, :Hq]); pages [L, pages, Hkv, page_size, D]."""
+    tokens, heads, D = qkv.shape
+    L, num_pages, Hkv, page_size, Dc = _pages(k_pages, v_pages, block_table, qkv.dtype)
+    Hq = heads - 2 * Hkv
+    B = _packed(cu_tokens, history_length, block_table)
+    if q_out.shape != (tokens, Hq, D) or Dc != D or q_out.dtype != qkv.dtype:
+        raise ValueError("q_out [tokens, Hq, D] of qkv's type and the pages' head size expected")
+    if bias is not None and (bias.numel() != heads * D or bias.dtype != qkv.dtype):
+        raise ValueError("bias [(Hq+2Hkv)*D] of qkv's type expected")
+    _same_device(q_out, k_pages, v_pages, qkv, bias, cu_tokens, history_length, block_table)
+    _int32(cu_tokens, history_length, block_table)
+    qp, qs = _rows(q_out, "q_out")
+    if q_out.data_ptr() == qkv.data_ptr() and tokens == 1:
+        qs = heads * D
+    _check(lib().onellm_paged_qkv_store(_dt(qkv), qp, qs, _ptr(k_pages), _ptr(v_pages), _ptr(qkv), _ptr(bias), _ptr(cu_tokens),
+                                        _ptr(history_length), _ptr(block_table), B, tokens, Hq, Hkv, D, page_size, num_pages,
+                                        block_table.shape[1], layer, L, rotary_dim, rope_base, _stream()), "onellm_paged_qkv_store")
+    return q_out
+
+
+def paged_prompt_attn_workspace_bytes(B, token_num, Hq, Hkv, D, max_rows):
+    return lib().onellm_paged_prompt_attn_workspace_bytes(B, token_num, Hq, Hkv, D, max_rows)
+
+
+def paged_prompt_attn(q, k_pages, v_pages, out, cu_tokens, history_length, block_table, max_rows, layer=0, workspace=None):
+    """q, out [tokens, Hq, D], tokens may be a stride apart; pages [L, pages, Hkv, page_size, D]; max_rows: upper bound of a
+    sequence's history + tokens.  `workspace`: uint8 device tensor; allocated here when None."""
+    import torch
+    tokens, Hq, D = q.shape
+    L, num_pages, Hkv, page_size, Dc = _pages(k_pages, v_pages, block_table, q.dtype)
+    B = _packed(cu_tokens, history_length, block_table)
+    if out.shape != q.shape or Dc != D or out.dtype != q.dtype:
+        raise ValueError("out like q and the pages' head size expected")
+    _same_device(q, k_pages, v_pages, out, cu_tokens, history_length, block_table, workspace)
+    _int32(cu_tokens, history_length, block_table)
+    if workspace is None:
+        workspace = torch.empty(paged_prompt_attn_workspace_bytes(B, tokens, Hq, Hkv, D, int(max_rows)), dtype=torch.uint8,
+                                device=q.device)
+    qp, qs = _rows(q, "q")
+    op, os_ = _rows(out, "out")
+    _check(lib().onellm_paged_prompt_attn(_dt(q), qp, qs, _ptr(k_pages), _ptr(v_pages), op, os_, _ptr(cu_tokens),
+                                          _ptr(history_length), _ptr(block_table), B, tokens, Hq, Hkv, D, page_size, num_pages,
+                                          block_table.shape[1], layer, L, int(max_rows), _ptr(workspace), workspace.numel(),
+                                          _stream()), "onellm_paged_prompt_attn")
+    return out
 
 
 # ---------------------------------------------------------------- projection GEMMs (include/onellm_gemm.h)

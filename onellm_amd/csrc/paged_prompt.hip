@@ -1,0 +1,588 @@
+// Attention of packed prompt tokens over a paged key-value cache: causal, grouped heads, sequences of different lengths.
+//
+//   o[i] = sum_j softmax_j(q[i] . k[j] / sqrt(D)) v[j]   over rows j <= history + i of the token's sequence
+//
+// One pass over the rows with a running maximum and sum.  The query heads that share a kv head and the tokens of a sequence
+// are one axis (row m = token * G + head), so a tile of 128 rows reads K and V once for all of them.
+//
+// A wave owns 32 rows.  It computes the transposed score tile S^T = K Q^T: in the result layout of the 32 x 32 products a
+// lane then holds 16 of the 32 keys' scores of ONE row (the other half is in lane ^ 32), so the softmax needs a single
+// lane exchange per tile, and the registers it leaves are, as they stand, the B operand of O^T = V^T P^T: product i takes
+// the keys its lanes hold, and V^T's operand picks the same keys.  For fp16 that operand (a column of V over four
+// keys) comes out of the LDS transposed (ds_read_b64_tr_b16); for fp32 a product takes two keys and reads them as they are.
+// Scores, statistics and output are fp32.  fp16: P enters its product rounded to fp16 (half a step, 2^-12 relative of each
+// weight, averaged over the keys); the sum of the weights is taken before that rounding.
+#include "paged.hpp"
+
+namespace onellm {
+namespace {
+
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kRowsPerTile = 128, kThreads = 256;
+
+struct PromptArgs {
+    const void* q;
+    const void* k_pages;
+    const void* v_pages;
+    void* out;
+    const int* cu;
+    const int* hist;
+    PagedCache cache;
+    long q_stride, out_stride;
+    int B, token_num, Hq, G;
+    float score_scale;         // log2(e) / sqrt(D)
+    int nsplit, chunk;         // pieces a tile's rows of the cache are cut into, rows per piece (the last takes the rest)
+    float* part_o;             // [nsplit, token_num * Hq, D]
+    float* part_ml;            // [nsplit, token_num * Hq, 2]
+};
+
+// The tile a workgroup works on: tiles are numbered sequence by sequence, the last (longest) tile of the last sequence first.
+struct Tile {
+    int b, first, len, hist;   // sequence, its first packed token, tokens, rows before them
+    int m0;                    // first row of the tile: token m / G, head m % G of the group
+};
+
+__device__ __forceinline__ int tiles_of(const PromptArgs& a, int b, int& first, int& len)
+{
+    first = max(a.cu[b], 0);
+    len = min(a.cu[b + 1], a.token_num) - first;
+    if (len <= 0 || a.hist[b] < 0) return 0;
+    return (len * a.G + kRowsPerTile - 1) / kRowsPerTile;
+}
+
+__device__ __forceinline__ bool locate_tile(const PromptArgs& a, int index, Tile& t)
+{
+    const int lane = threadIdx.x & (kWave - 1);
+    int total = 0;
+    for (int c = 0; c < a.B; c += kWave) {
+        int first, len;
+        int n = c + lane < a.B ? tiles_of(a, c + lane, first, len) : 0;
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o, kWave);
+        total += n;
+    }
+    if (index >= total) return false;
+    const int want = total - 1 - index;
+    int run = 0;
+    for (int c = 0; c < a.B; c += kWave) {
+        int first = 0, len = 0;
+        const int n = c + lane < a.B ? tiles_of(a, c + lane, first, len) : 0;
+        int inc = n;
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const int up = __shfl_up(inc, o, kWave);
+            if (lane >= o) inc += up;
+        }
+        const int tot = __shfl(inc, kWave - 1, kWave);
+        if (want < run + tot) {
+            const int f = __builtin_ctzll(__builtin_amdgcn_ballot_w64(run + inc > want));
+            t.b = c + f;
+            t.first = __shfl(first, f, kWave);
+            t.len = __shfl(len, f, kWave);
+            t.m0 = (want - run - __shfl(inc - n, f, kWave)) * kRowsPerTile;
+            t.hist = min(a.hist[t.b], 1 << 30);    // (past every table: all its rows are seen)
+            return true;
+        }
+        run += tot;
+    }
+    return false;
+}
+
+constexpr unsigned kOutside = 0x7FFFFF00u;     // a byte offset no window of 16 rows reaches
+
+template <typename T, int DP>
+struct PromptShape {
+    static constexpr bool kHalf = sizeof(T) == 2;
+    static constexpr int VEC = 16 / sizeof(T);
+    static constexpr int BN = kHalf && DP <= 128 ? 64 : 32; // keys per step
+    static constexpr int P = DP / VEC;                      // 16-byte pieces of a staged row
+    static constexpr int ROW = DP * (int)sizeof(T);         // bytes of a staged row
+    static constexpr int LD = BN * P / kThreads;            // pieces per thread and operand
+    static constexpr int NG = BN / kRowGroup;               // row groups per step
+    static constexpr int NS = BN / 32;                      // score tiles per step
+    static constexpr int ND = DP / 32;                      // output tiles
+    static constexpr int TILE = BN * ROW;                   // bytes of a staged operand
+    static_assert(BN * P % kThreads == 0 && (kWave / P <= kRowGroup), "whole pieces per thread; a wave's pieces lie in one row group");
+    // LDS keeps piece p of row r at p ^ swizzle(r): without it the lanes of a read, which take one piece each of
+    // 16 or more rows, would all hit the same banks
+    __device__ static __forceinline__ int swz_k(int r) { return P == 8 ? (r >> 1) & 7 : r & 15; }
+    __device__ static __forceinline__ int swz_v(int r)
+    {
+        if constexpr (!kHalf) return ((r >> 2) & 1) * 8;
+        else return P == 8 ? ((r >> 1) & 3) << 1 : (r & 7) << 1;
+    }
+};
+
+// four consecutive elements out of a window (zeros behind its end)
+template <typename T> struct Quad { T v[4]; };
+template <typename T>
+__device__ __forceinline__ Quad<T> load_quad(__amdgpu_buffer_rsrc_t w, int offset)
+{
+    if constexpr (sizeof(T) == 2) return __builtin_bit_cast(Quad<T>, __builtin_amdgcn_raw_buffer_load_b64(w, offset, 0, 0));
+    else return __builtin_bit_cast(Quad<T>, __builtin_amdgcn_raw_buffer_load_b128(w, offset, 0, 0));
+}
+
+__device__ __forceinline__ float other_half_max(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void prompt_tile(const PromptArgs& a)
+{
+    using S = PromptShape<T, DP>;
+    constexpr int VEC = S::VEC, BN = S::BN, P = S::P, LD = S::LD, NS = S::NS, ND = S::ND;
+    // (four arrays, not one: the compiler then sees that the rows on their way to one pair do not touch the other)
+    __shared__ __align__(16) char k_even[S::TILE], v_even[S::TILE], k_odd[S::TILE], v_odd[S::TILE];
+    __shared__ unsigned s_bad[3][2];                // keys of a masked step whose V row holds a NaN or an infinity
+
+    Tile t;
+    if (!locate_tile(a, blockIdx.y, t)) return;
+    // the same in every lane: said here, behind the search's loops, so that all that follows from it stays scalar
+    t.b = __builtin_amdgcn_readfirstlane(t.b);
+    t.first = __builtin_amdgcn_readfirstlane(t.first);
+    t.len = __builtin_amdgcn_readfirstlane(t.len);
+    t.hist = __builtin_amdgcn_readfirstlane(t.hist);
+    t.m0 = __builtin_amdgcn_readfirstlane(t.m0);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int kvh = blockIdx.x, D = a.cache.D;
+    const int M = t.len * a.G;
+    const int m = t.m0 + wave * 32 + col;           // this lane's row
+    const bool row_ok = m < M;
+    const int token = row_ok ? m / a.G : 0, head = kvh * a.G + (row_ok ? m % a.G : 0);
+    // (a division leaves its quotient in a vector register: back to a scalar one, with all that follows from it)
+    const int last = __builtin_amdgcn_readfirstlane(min((t.m0 + kRowsPerTile - 1) / a.G, t.len - 1));
+    const int rows_end = min(t.hist + last + 1, a.cache.max_pages << a.cache.page_shift);       // rows any row of the tile sees
+    const int rows_all = t.hist + __builtin_amdgcn_readfirstlane(t.m0 / a.G) + 1;               // rows every row of it sees
+    const int k_begin = blockIdx.z * a.chunk;
+    const int k_end = blockIdx.z + 1 == (unsigned)a.nsplit ? rows_end : min(k_begin + a.chunk, rows_end);
+    const int limit = min(t.hist + token, k_end - 1);      // the last key the row sees (the table may end before its position)
+    const int* table = a.cache.table + (size_t)t.b * a.cache.max_pages;
+
+    // Q: lane (col, half) holds pieces 2 k + half of its row
+    Vec16<T> qf[P / 2];
+    {
+        const T* q = static_cast<const T*>(a.q) + (size_t)(t.first + token) * a.q_stride + (size_t)head * D;
+#pragma unroll
+        for (int k = 0; k < P / 2; ++k) {
+            const int p = 2 * k + half;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) qf[k].set(e, 0.f);
+            if (row_ok && p * VEC < D) qf[k] = load16(q + p * VEC);
+        }
+    }
+
+    if (tid < 6) s_bad[tid / 2][tid % 2] = 0;
+    float mx = -INFINITY, l = 0.f;                  // of this lane's row; l over the keys this lane holds
+    f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+
+    typedef int Pages __attribute__((ext_vector_type(4)));
+    Pages pages = {0, 0, 0, 0};                     // of the row groups of the step that is requested next
+    static_assert(S::NG <= 4, "row groups per step");
+    auto fetch_pages = [&](int k0) __attribute__((always_inline)) {
+        auto one = [&](int row) __attribute__((always_inline)) {
+            return row < k_end ? __builtin_amdgcn_readfirstlane(page_of(a.cache, table, row)) : 0;
+        };
+        pages.x = one(k0);
+        pages.y = one(k0 + kRowGroup);
+        if constexpr (S::NG > 2) {
+            pages.z = one(k0 + 2 * kRowGroup);
+            pages.w = one(k0 + 3 * kRowGroup);
+        }
+    };
+    // Rows k0 .. k0 + BN - 1 go straight from memory to LDS, 16 bytes per lane: slot (tid + 256 i) is (row, p') and
+    // gets piece p' ^ swizzle(row).  A wave's slots lie in one group of 16 rows, which is read through a window that holds
+    // the rows the sequence has there: rows behind its end, rows on a page that is none, and pieces behind the head's
+    // end arrive as zeros.
+    auto request = [&](char* kb, char* vb, int k0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int row = (i * kThreads + tid) / P, p = (i * kThreads + tid) % P;
+            const int g0 = (i * kThreads + wave * 64) / P / kRowGroup;       // (the wave's group)
+            int page = pages.x;
+            if constexpr (S::NG > 1) page = g0 == 1 ? pages.y : page;
+            if constexpr (S::NG > 2) page = g0 == 2 ? pages.z : (g0 == 3 ? pages.w : page);
+            const int row0 = k0 + g0 * kRowGroup;
+            const int rows = page < 0 ? 0 : min(max(k_end - row0, 0), kRowGroup);
+            const size_t at = paged_offset(a.cache, max(page, 0), kvh, row0);
+            const int bytes = rows * D * (int)sizeof(T);
+            T* kp = const_cast<T*>(static_cast<const T*>(a.k_pages)) + at;
+            T* vp = const_cast<T*>(static_cast<const T*>(a.v_pages)) + at;
+            const unsigned line = (unsigned)((row % kRowGroup) * D) * (unsigned)sizeof(T);
+            const int pk = p ^ S::swz_k(row), pv = p ^ S::swz_v(row);
+            typedef __attribute__((address_space(3))) void lds_void;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(kp, 0, bytes, 0x00020000),
+                                                     (lds_void*)(kb + (i * kThreads + wave * 64) * 16), 16,
+                                                     pk * VEC < D ? line + pk * 16 : kOutside, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(vp, 0, bytes, 0x00020000),
+                                                     (lds_void*)(vb + (i * kThreads + wave * 64) * 16), 16,
+                                                     pv * VEC < D ? line + pv * 16 : kOutside, 0, 0, 0);
+        }
+    };
+    // Masked steps: a NaN or an infinity in a V row would reach rows that do not see it (0 * NaN), so every thread
+    // replaces those among the pieces it brought by zeros and notes their keys; compute() adds them to the rows that do see them.
+    auto clean = [&](char* vb, int slot) __attribute__((always_inline)) {
+#pragma unroll 1
+        for (int i = 0; i < LD; ++i) {
+            Vec16<T>* at = reinterpret_cast<Vec16<T>*>(vb + (i * kThreads + tid) * 16);
+            Vec16<T> v = *at;
+            bool bad = false;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const bool fin = __builtin_fabsf(v.get(e)) < INFINITY;
+                bad = bad || !fin;
+                v.set(e, fin ? v.get(e) : 0.f);
+            }
+            if (bad) {
+                *at = v;
+                const int row = (i * kThreads + tid) / P;
+                atomicOr(&s_bad[slot][row / 32], 1u << (row % 32));
+            }
+        }
+    };
+
+    // one step: keys k0 .. k0 + BN - 1.  valid: bit g = group g's page exists (masked steps only)
+    auto compute = [&](const char* kb, const char* vb, int k0, auto masked_tag, unsigned valid, int slot) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked_tag)::value;
+        f32x16 s[NS];
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
+            const int row = n * 32 + col;
+#pragma unroll
+            for (int k = 0; k < P / 2; ++k) {
+                Vec16<T> kf;
+                kf.raw = *reinterpret_cast<const decltype(kf.raw)*>(kb + row * S::ROW + ((2 * k + half) ^ S::swz_k(row)) * 16);
+                if constexpr (S::kHalf) {
+                    s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf.raw, qf[k].raw, s[n], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.raw[e], qf[k].raw[e], s[n], 0, 0, 0);
+                }
+            }
+        }
+        if constexpr (MASKED) {
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = n * 32 + 8 * (r / 4) + 4 * half + r % 4;
+                    const bool see = k0 + key <= limit && (valid >> (n * 2 + r / 8) & 1u);
+                    s[n][r] = see ? s[n][r] : -INFINITY;
+                }
+        }
+        float bm = s[0][0];
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) bm = fmaxf(bm, s[n][r]);
+        bm = other_half_max(bm);
+        if (__builtin_amdgcn_ballot_w64(bm > mx) != 0) {
+            const float mnew = fmaxf(mx, bm);
+            const float alpha = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mx - mnew) * a.score_scale);
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+            mx = mnew;
+        }
+        const float shift = mx == -INFINITY ? 0.f : mx * a.score_scale;      // (a row that has seen nothing yet)
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.score_scale, -shift));
+                l += s[n][r];
+            }
+        if constexpr (S::kHalf) {
+#pragma unroll
+            for (int i = 0; i < BN / 16; ++i) {
+                // keys 16 i + 8 (e / 4) + 4 half + e % 4: what the score registers 8 (i % 2) .. + 7 of this lane are
+                f16x8 pf;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) pf[e] = (_Float16)s[i / 2][8 * (i % 2) + e];
+                // 16 lanes read four rows x 16 columns, four elements each, and get one column of the four rows each
+                const int row = 16 * i + 4 * half + (lane & 15) / 4;
+                const int row2 = row + 8;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const int piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4*)(vb + row * S::ROW + (piece ^ S::swz_v(row)) * 16 + (lane & 1) * 8));
+                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4*)(vb + row2 * S::ROW + (piece ^ S::swz_v(row2)) * 16 + (lane & 1) * 8));
+                    const f16x8 vf = __builtin_bit_cast(f16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf, o[d], 0, 0, 0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int row = n * 32 + 8 * (r / 4) + 4 * half + r % 4;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        const int piece = 8 * d + col / 4;
+                        const float vf = *reinterpret_cast<const float*>(vb + row * S::ROW + (piece ^ S::swz_v(row)) * 16 + (col % 4) * 4);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[n][r], o[d], 0, 0, 0);
+                    }
+                }
+        }
+        if constexpr (MASKED) {
+            // (rare) keys with a NaN or an infinity in V: added to the rows that see them.  A weight of any size times
+            // such a value is that value.
+#pragma unroll 1
+            for (int w = 0; w < (BN + 31) / 32; ++w) {
+                unsigned bits = __builtin_amdgcn_readfirstlane(s_bad[slot][w]);
+#pragma unroll 1
+                while (bits) {
+                    const int key = k0 + w * 32 + __builtin_ctz(bits);
+                    bits &= bits - 1;
+                    const int page = __builtin_amdgcn_readfirstlane(page_of(a.cache, table, key));
+                    if (page < 0) continue;
+                    const T* v = static_cast<const T*>(a.v_pages) + paged_offset(a.cache, page, kvh, key);
+                    const __amdgpu_buffer_rsrc_t w = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(v), 0, D * (int)sizeof(T), 0x00020000);
+                    const bool see = key <= limit;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int r4 = 0; r4 < 4; ++r4) {
+                            const Quad<T> x = load_quad<T>(w, (32 * d + 8 * r4 + 4 * half) * (int)sizeof(T));
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float f = to_f32(x.v[e]);
+                                o[d][4 * r4 + e] += see && !(__builtin_fabsf(f) < INFINITY) ? f : 0.f;
+                            }
+                            __builtin_amdgcn_sched_barrier(0);       // (four values at a time: no registers for a path this rare)
+                        }
+                }
+            }
+        }
+    };
+
+    if (k_begin < k_end) {
+        const int steps = (k_end - k_begin + BN - 1) / BN;
+        const int plain = max(0, min(k_end, rows_all) - k_begin) / BN;     // steps that every row of the tile sees whole
+        constexpr unsigned kAll = (1u << S::NG) - 1u;
+        unsigned valid = 0;
+        bool masked = false;
+        int it = 0;
+        auto look = [&](int step) __attribute__((always_inline)) {                 // what the pages of a step say about it
+            valid = (pages.x >= 0 ? 1u : 0u) | (pages.y >= 0 ? 2u : 0u);
+            if constexpr (S::NG > 2) valid |= (pages.z >= 0 ? 4u : 0u) | (pages.w >= 0 ? 8u : 0u);
+            masked = step >= plain || valid != kAll;
+        };
+        auto arrive = [&](char* vb, int slot) __attribute__((always_inline)) {     // this wave's rows are there; then everybody's
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (masked) clean(vb, slot);
+            __syncthreads();
+        };
+        auto step = [&](char* kb, char* vb, char* kn, char* vn) __attribute__((always_inline)) {
+            const int k0 = k_begin + it * BN;
+            const unsigned valid_now = valid;
+            const bool masked_now = masked, more = it + 1 < steps;
+            if (more) {
+                request(kn, vn, k0 + BN);
+                look(it + 1);
+                fetch_pages(k0 + 2 * BN);
+            }
+            if (masked_now) compute(kb, vb, k0, std::true_type{}, valid_now, it % 3);
+            else compute(kb, vb, k0, std::false_type{}, kAll, 0);
+            if (more) {
+                if (tid < 2) s_bad[(it + 2) % 3][tid] = 0;       // (last read before the previous barrier, next written behind the coming one)
+                arrive(vn, (it + 1) % 3);
+            }
+            ++it;
+            return more;
+        };
+        fetch_pages(k_begin);
+        request(k_even, v_even, k_begin);
+        look(0);
+        fetch_pages(k_begin + BN);
+        __syncthreads();                                         // s_bad is clear
+        arrive(v_even, 0);
+        while (step(k_even, v_even, k_odd, v_odd) && step(k_odd, v_odd, k_even, v_even)) {}
+    }
+
+    l += __shfl_xor(l, 32, kWave);
+    if (!row_ok) return;
+    if (a.nsplit > 1) {
+        const size_t e = (size_t)blockIdx.z * ((size_t)a.token_num * a.Hq) + (size_t)(t.first + token) * a.Hq + head;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const int c = 32 * d + 8 * r4 + 4 * half;
+                if (c < D) *reinterpret_cast<f32x4*>(a.part_o + e * D + c) = f32x4{o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]};
+            }
+        if (half == 0) {
+            a.part_ml[e * 2] = mx;
+            a.part_ml[e * 2 + 1] = l;
+        }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;            // (a row that sees no key: zeros)
+    T* out = static_cast<T*>(a.out) + (size_t)(t.first + token) * a.out_stride + (size_t)head * D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const int c = 32 * d + 8 * r4 + 4 * half;
+            if (c < D) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out[c + e] = from_f32<T>(o[d][4 * r4 + e] * inv);
+            }
+        }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1)
+void paged_prompt_attn_kernel(const PromptArgs a)
+{
+    prompt_tile<T, DP>(a);
+}
+
+// Joins the pieces of a split step: one workgroup row per (token, head), four columns per thread.
+template <typename T>
+__global__ __launch_bounds__(256)
+void paged_prompt_merge_kernel(const PromptArgs a)
+{
+    const int nq = a.cache.D / 4;                          // (D is a multiple of four)
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    const long rows = (long)a.token_num * a.Hq;
+    if (i >= rows * nq) return;
+    const long row = i / nq;
+    const int c = (int)(i % nq) * 4;
+    const int token = (int)(row / a.Hq), head = (int)(row % a.Hq);
+    // whose token is it?  (a token of no sequence has no partial states and keeps its output)
+    int lo = 0, hi = a.B;                                  // the first b with cu[b + 1] > token
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (a.cu[mid + 1] <= token) lo = mid + 1;
+        else hi = mid;
+    }
+    if (lo >= a.B || token < a.cu[lo] || a.hist[lo] < 0) return;
+    float M = -INFINITY;
+    for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, a.part_ml[(s * rows + row) * 2]);
+    float L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.nsplit; ++s) {
+        const float m = a.part_ml[(s * rows + row) * 2];
+        if (m == -INFINITY) continue;                      // a piece that saw nothing
+        const float w = __builtin_amdgcn_exp2f((m - M) * a.score_scale);
+        L = __builtin_fmaf(a.part_ml[(s * rows + row) * 2 + 1], w, L);
+        const f32x4 p = *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * a.cache.D + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) O[e] = __builtin_fmaf(p[e], w, O[e]);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    T* out = static_cast<T*>(a.out) + (size_t)token * a.out_stride + (size_t)head * a.cache.D + c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = from_f32<T>(O[e] * inv);
+}
+
+template <typename T>
+int launch_prompt(const PromptArgs& a, int tiles, hipStream_t st)
+{
+    const dim3 grid(a.cache.Hkv, tiles, a.nsplit);
+    if (a.cache.D <= 64) hipLaunchKernelGGL((paged_prompt_attn_kernel<T, 64>), grid, dim3(kThreads), 0, st, a);
+    else if (a.cache.D <= 128) hipLaunchKernelGGL((paged_prompt_attn_kernel<T, 128>), grid, dim3(kThreads), 0, st, a);
+    else hipLaunchKernelGGL((paged_prompt_attn_kernel<T, 256>), grid, dim3(kThreads), 0, st, a);
+    int rc = launch_status();
+    if (rc || a.nsplit == 1) return rc;
+    const long n = (long)a.token_num * a.Hq * (a.cache.D / 4);
+    hipLaunchKernelGGL((paged_prompt_merge_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    return launch_status();
+}
+
+// tiles of all sequences, at most (every sequence may end in a tile of its own)
+long tiles_bound(int B, int token_num, int G)
+{
+    const long rows = (long)token_num * G;
+    return rows / kRowsPerTile + (token_num < B ? token_num : B);
+}
+
+// Pieces the rows of the cache are cut into: none while the tiles alone fill the chip (two workgroups per compute unit),
+// else as many as fill it, of 512 rows or more each.
+int split_of(long tiles, int Hkv, int max_rows)
+{
+    const long wgs = tiles * Hkv;
+    long n = 512 / (wgs < 1 ? 1 : wgs);
+    const long most = max_rows / 512;
+    if (n > most) n = most;
+    return n < 1 ? 1 : (int)n;
+}
+
+}  // namespace
+}  // namespace onellm
+
+extern "C" size_t onellm_paged_prompt_attn_workspace_bytes(int B, int token_num, int Hq, int Hkv, int D, int max_rows)
+{
+    using namespace onellm;
+    if (B <= 0 || token_num <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || max_rows <= 0) return 256;
+    const int n = split_of(tiles_bound(B, token_num, Hq / Hkv), Hkv, max_rows);
+    if (n == 1) return 256;
+    return (((size_t)n * token_num * Hq * (D + 2) * sizeof(float)) + 255) / 256 * 256;
+}
+
+extern "C" int onellm_paged_prompt_attn(int dtype, const void* q, long q_stride, const void* k_pages, const void* v_pages, void* out,
+                                        long out_stride, const int* cu_tokens, const int* history_length, const int* block_table,
+                                        int B, int token_num, int Hq, int Hkv, int D, int page_size, int num_pages, int max_pages,
+                                        int layer, int num_layers, int max_rows, void* workspace, size_t workspace_bytes,
+                                        onellm_stream_t stream)
+{
+    using namespace onellm;
+    const int rc = check_paged(dtype, k_pages, v_pages, block_table, B, Hq, Hkv, D, page_size, num_pages, max_pages, layer, num_layers);
+    if (rc) return rc;
+    if (token_num < 0 || !cu_tokens || !history_length) return ONELLM_EINVAL;
+    if (max_rows <= 0) return ONELLM_EINVAL;
+    if (token_num == 0) return 0;
+    if (!q || !out) return ONELLM_EINVAL;
+    const int vec = dtype == ONELLM_FP16 ? 8 : 4;
+    if (q_stride < (long)Hq * D || out_stride < (long)Hq * D) return ONELLM_EINVAL;
+    if (!aligned16(q) || !aligned16(out) || q_stride % vec != 0 || out_stride % vec != 0) return ONELLM_EUNSUPPORTED;
+    const int G = Hq / Hkv;
+    const long tiles = tiles_bound(B, token_num, G);
+    if ((long)token_num * Hq > 0x3FFFFFFFL || tiles > 65535) return ONELLM_EUNSUPPORTED;
+    PromptArgs a;
+    a.q = q;
+    a.k_pages = k_pages;
+    a.v_pages = v_pages;
+    a.out = out;
+    a.cu = cu_tokens;
+    a.hist = history_length;
+    a.cache = make_paged(block_table, max_pages, num_pages, page_size, Hkv, D, layer);
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.B = B;
+    a.token_num = token_num;
+    a.Hq = Hq;
+    a.G = G;
+    a.score_scale = 1.44269504088896340736f / sqrtf((float)D);
+    a.nsplit = split_of(tiles, Hkv, max_rows);
+    a.chunk = ((max_rows + a.nsplit - 1) / a.nsplit + 63) / 64 * 64;
+    a.part_o = nullptr;
+    a.part_ml = nullptr;
+    if (a.nsplit > 1) {
+        if (!workspace || workspace_bytes < onellm_paged_prompt_attn_workspace_bytes(B, token_num, Hq, Hkv, D, max_rows)
+            || !aligned16(workspace)) return ONELLM_EWORKSPACE;
+        a.part_o = static_cast<float*>(workspace);
+        a.part_ml = a.part_o + (size_t)a.nsplit * token_num * Hq * D;
+    }
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return dtype == ONELLM_FP16 ? launch_prompt<__half>(a, (int)tiles, st) : launch_prompt<float>(a, (int)tiles, st);
+}
