@@ -326,6 +326,30 @@ int onellm_paged_prompt_attn(int dtype, const void* q, long q_stride, const void
                              int max_rows, void* workspace, size_t workspace_bytes, onellm_stream_t stream);
 size_t onellm_paged_prompt_attn_workspace_bytes(int B, int token_num, int Hq, int Hkv, int D, int max_rows);
 
+/*
+ * Decode attention for ONE new token per sequence over the paged cache: onellm_decode_attn's step (QKV bias, rotary position,
+ * the new k and v row into the cache, attention over the sequence's rows and the new one) with the rows in pages.
+ *   qkv [B, Hq + 2 Hkv, D], qkv_bias as in onellm_decode_attn (may be NULL); out [B, Hq, D]
+ *   t_dev device int32[B]: attended positions including the new token, which sits at position t - 1; a sequence whose length
+ *         lies outside [1, min(max_t, max_pages * page_size)] is left alone, out row and cache included
+ *   max_t upper bound of the lengths
+ *   flags ONELLM_ATTN_ZEROED_WORKSPACE or 0.  The workspace starts with arrival counters that every call leaves at zero; with
+ *         the flag the caller states that it zero-filled the workspace once and that nothing but this entry point has written
+ *         it since, without it the call clears them first (one more launch)
+ *   workspace, workspace_bytes  onellm_paged_decode_attn_workspace_bytes(), 256-byte aligned; calls of different shapes may
+ *         share one (a zero-filled one too), calls that overlap in time may not
+ * History rows without a page take no part; the new token's own row always does, and is stored where it has a page.  The
+ * new rows are rounded to the cache's type before they take part; all arithmetic is fp32 or better.  The result does not
+ * depend on the order in which workgroups finish.
+ */
+int onellm_paged_decode_attn(int dtype, const void* qkv, const void* qkv_bias, void* k_pages, void* v_pages, void* out,
+                             const int* block_table, const int* t_dev,
+                             int B, int Hq, int Hkv, int D,
+                             int page_size, int num_pages, int max_pages, int layer, int num_layers,
+                             int max_t, int rotary_dim, float rope_base, unsigned flags,
+                             void* workspace, size_t workspace_bytes, onellm_stream_t stream);
+size_t onellm_paged_decode_attn_workspace_bytes(int B, int Hq, int Hkv, int D, int max_t);
+
 #ifdef __cplusplus
 }
 #endif

@@ -48,6 +48,8 @@ SYMBOLS = {
     "onellm_topk_sample": (_ci, [_vp, _vp, _vp, _vp, _vp, _ci, _ci, ctypes.c_ulonglong, _ci, _ci, _vp]),
     "onellm_paged_qkv_store": (_ci, [_ci, _vp, _cl, _vp, _vp, _vp, _vp, _vp, _vp, _vp] + [_ci] * 11 + [_cf, _vp]),
     "onellm_paged_prompt_attn": (_ci, [_ci, _vp, _cl, _vp, _vp, _vp, _cl, _vp, _vp, _vp] + [_ci] * 11 + [_vp, _sz, _vp]),
+    "onellm_paged_decode_attn": (_ci, [_ci] + [_vp] * 7 + [_ci] * 11 + [_cf, _cu, _vp, _sz, _vp]),
+    "onellm_paged_decode_attn_workspace_bytes": (_sz, [_ci, _ci, _ci, _ci, _ci]),
     "onellm_paged_prompt_attn_workspace_bytes": (_sz, [_ci, _ci, _ci, _ci, _ci, _ci]),
 }
 
@@ -336,6 +338,34 @@ def paged_prompt_attn(q, k_pages, v_pages, out, cu_tokens, history_length, block
                                           _ptr(history_length), _ptr(block_table), B, tokens, Hq, Hkv, D, page_size, num_pages,
                                           block_table.shape[1], layer, L, int(max_rows), _ptr(workspace), workspace.numel(),
                                           _stream()), "onellm_paged_prompt_attn")
+    return out
+
+
+def paged_decode_attn_workspace_bytes(B, Hq, Hkv, D, max_t):
+    return lib().onellm_paged_decode_attn_workspace_bytes(B, Hq, Hkv, D, max_t)
+
+
+def paged_decode_attn(qkv, bias, k_pages, v_pages, out, block_table, t_dev, max_t, rotary_dim, rope_base, layer=0, flags=0,
+                      workspace=None):
+    """qkv [B, Hq+2Hkv, D]; pages [L, pages, Hkv, page_size, D]; out [B, Hq, D]; t_dev int32 [B], lengths with the new token,
+    at most max_t.  `workspace`: uint8 device tensor; allocated here when None."""
+    import torch
+    B, heads, D = qkv.shape
+    L, num_pages, Hkv, page_size, Dc = _pages(k_pages, v_pages, block_table, qkv.dtype)
+    Hq = heads - 2 * Hkv
+    if out.shape != (B, Hq, D) or Dc != D or out.dtype != qkv.dtype or t_dev.numel() != B or block_table.shape[0] != B:
+        raise ValueError("out [B, Hq, D] of qkv's type, t_dev [B], block_table [B, max_pages] and the pages' head size expected")
+    if bias is not None and (bias.numel() != heads * D or bias.dtype != qkv.dtype):
+        raise ValueError("bias [(Hq+2Hkv)*D] of qkv's type expected")
+    _same_device(qkv, bias, k_pages, v_pages, out, block_table, t_dev, workspace)
+    _int32(block_table, t_dev)
+    if workspace is None:
+        workspace = torch.empty(paged_decode_attn_workspace_bytes(B, Hq, Hkv, D, int(max_t)), dtype=torch.uint8, device=qkv.device)
+        flags &= ~ATTN_ZEROED_WORKSPACE
+    _check(lib().onellm_paged_decode_attn(_dt(qkv), _ptr(qkv), _ptr(bias), _ptr(k_pages), _ptr(v_pages), _ptr(out),
+                                          _ptr(block_table), _ptr(t_dev), B, Hq, Hkv, D, page_size, num_pages,
+                                          block_table.shape[1], layer, L, int(max_t), rotary_dim, rope_base, flags,
+                                          _ptr(workspace), workspace.numel(), _stream()), "onellm_paged_decode_attn")
     return out
 
 

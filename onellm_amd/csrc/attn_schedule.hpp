@@ -1,5 +1,5 @@
 // Decode attention: launch arguments, what a workgroup works on, the grid and the balanced workgroup schedules.
-// (part of decode_attn.hip, which is the only file that includes it: everything here sits in its anonymous namespace)
+// (part of decode_attn.hip and paged_decode.hip: everything here sits in the anonymous namespace of the file that includes it)
 #pragma once
 #include "common.hpp"
 

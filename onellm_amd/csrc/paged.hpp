@@ -27,8 +27,17 @@ __device__ __forceinline__ int page_of(const PagedCache& c, const int* table_row
 {
     const int p = row >> c.page_shift;
     if (p >= c.max_pages) return -1;
-    const int id = table_row[p];
+    // (nothing writes the table while a kernel runs: read as constant memory, by the scalar unit where p is uniform)
+    typedef const __attribute__((address_space(4))) int const_int;
+    const int id = ((const_int*)reinterpret_cast<uintptr_t>(table_row))[p];
     return (unsigned)id < (unsigned)c.num_pages ? id : -1;
+}
+
+// rows of the group at row0 that lie in front of `end` (both the same in every lane; the three-operand clamp only exists on the
+// vector unit, so its result is brought back to a scalar register: a memory window has to be one)
+__device__ __forceinline__ int rows_left(int end, int row0)
+{
+    return __builtin_amdgcn_readfirstlane(min(max(end - row0, 0), kRowGroup));
 }
 
 // element offset of row `row` (of the sequence) of kv head `kvh` in page `page`

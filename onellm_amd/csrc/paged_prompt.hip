@@ -213,7 +213,7 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
             if constexpr (S::NG > 1) page = g0 == 1 ? pages.y : page;
             if constexpr (S::NG > 2) page = g0 == 2 ? pages.z : (g0 == 3 ? pages.w : page);
             const int row0 = k0 + g0 * kRowGroup;
-            const int rows = page < 0 ? 0 : min(max(k_end - row0, 0), kRowGroup);
+            const int rows = page < 0 ? 0 : rows_left(k_end, row0);
             const size_t at = paged_offset(a.cache, max(page, 0), kvh, row0);
             const int bytes = rows * D * (int)sizeof(T);
             T* kp = const_cast<T*>(static_cast<const T*>(a.k_pages)) + at;

@@ -126,6 +126,29 @@ def prompt(q, k_pages, v_pages, cu, hist, table, layer):
     return out, tol, covered
 
 
+def decode(c, t_host, k_rows, v_rows, rotary_dim, base, bias=True):
+    """One new token per sequence of case c (its qkv's first rows).  k_rows, v_rows [B, Hkv, D]: the new rows as the cache holds
+    them.  Returns (out, tolerance) [B, Hq, D]; sequences of length 0 or less are left at zero."""
+    B = len(t_host)
+    x = c.qkv[:B].double()
+    if bias:
+        x = x + c.bias.double().view(c.hq + 2 * c.hkv, c.d)
+    out = torch.zeros(B, c.hq, c.d, dtype=torch.float64, device=c.q.device)
+    tol = torch.zeros_like(out)
+    for b, t in enumerate(t_host):
+        if t < 1:
+            continue
+        q = rotate(x[b:b + 1, :c.hq], torch.tensor([t - 1], device=c.q.device), rotary_dim, base)
+        k, there = rows_of(c.kp, c.layer, c.table, b, t)
+        v, _ = rows_of(c.vp, c.layer, c.table, b, t)
+        k[t - 1], v[t - 1], there[t - 1] = k_rows[b].double(), v_rows[b].double(), True
+        o, mean, size = attend(q, k, v, there, t - 1)
+        # on top of attention's: q is rotated in fp32 (2^-21 of a pair) and enters as two halves (2^-22)
+        out[b] = o[0]
+        tol[b] = (attention_tolerance(c.dtype, c.d, t, o, mean, size, float(v.abs().max())) + 2.0 ** -18 * size * mean)[0]
+    return out, tol
+
+
 class Case:
     """Random inputs of a packed batch over shuffled pages; rows no sequence has hold NaN"""
 

@@ -268,3 +268,203 @@ def test_prompt_on_other_streams_and_in_graphs(capi, dev):
         c.hist[0] -= 100
         c.hist_host[0] -= 100
         want[0] = check_prompt(capi, c)
+
+
+# ---------------------------------------------------------------- one new token per sequence
+
+def decode_case(dtype, ts, hq, hkv, d, ps, seed, **kw):
+    """sequences of ts[b] rows with the new token; its own row is not in the cache yet"""
+    c = pm.Case(dtype, [max(t, 1) for t in ts], [0] * len(ts), hq, hkv, d, ps, seed=seed, **kw)
+    c.ts = ts
+    c.qkv = c.qkv[:len(ts)].contiguous()
+    c.t_dev = torch.tensor(ts, dtype=torch.int32, device=c.q.device)
+    for b, t in enumerate(ts):
+        if t >= 1:
+            page = pm.page_of(c.table, b, t - 1, c.num_pages, ps)
+            c.kp[c.layer, page, :, (t - 1) % ps] = float("nan")
+            c.vp[c.layer, page, :, (t - 1) % ps] = float("nan")
+    return c
+
+
+def run_decode(capi, c, kp, vp, rotary_dim, base=10000.0, bias=True, max_t=None, flags=0, workspace=None, out=None):
+    announce("paged decode", c.dtype, c.ts, c.hq, c.hkv, c.d, c.ps, max_t, flags)
+    if out is None:
+        out = torch.full((len(c.ts), c.hq, c.d), MARK, dtype=c.dtype, device=c.q.device)
+    capi.paged_decode_attn(c.qkv, c.bias if bias else None, kp, vp, out, c.table, c.t_dev, max(1, max(c.ts)) if max_t is None else max_t,
+                           rotary_dim, base, layer=c.layer, flags=flags, workspace=workspace)
+    torch.cuda.synchronize()
+    return out
+
+
+def check_decode(capi, c, rotary_dim, base=10000.0, bias=True, skip=(), **kw):
+    """skip: sequences that have to be left alone"""
+    B = len(c.ts)
+    ts = [0 if b in skip else t for b, t in enumerate(c.ts)]
+    # the new rows, within a rounding of their definition
+    lens, hist = [1 if t >= 1 else 0 for t in ts], [max(0, t - 1) for t in ts]
+    cu = [sum(lens[:i]) for i in range(B + 1)]
+    keep = [b for b in range(B) if lens[b]]
+    _, written, _ = pm.store(c.qkv[keep], c.bias if bias else None, c.kp, c.vp, cu, hist, c.table, c.layer, rotary_dim, base)
+    kp, vp = c.kp.clone(), c.vp.clone()
+    out = run_decode(capi, c, kp, vp, rotary_dim, base, bias, **kw)
+    k_rows = torch.zeros(B, c.hkv, c.d, dtype=c.dtype, device=c.q.device)
+    v_rows = k_rows.clone()
+    for b in keep:
+        page = pm.page_of(c.table, b, c.ts[b] - 1, c.num_pages, c.ps)
+        row = (c.ts[b] - 1) % c.ps
+        if page < 0:                                        # not stored: what the same call stores where there is a page
+            other = pm.Case(c.dtype, [c.ts[b]], [0], c.hq, c.hkv, c.d, c.ps, device=c.q.device, seed=1)
+            other.qkv, other.bias, other.ts, other.layer = c.qkv[b:b + 1].contiguous(), c.bias, [c.ts[b]], 0
+            other.t_dev = c.t_dev[b:b + 1].contiguous()
+            run_decode(capi, other, other.kp, other.vp, rotary_dim, base, bias)
+            k_rows[b], v_rows[b] = (x[0, int(other.table[0, (c.ts[b] - 1) // c.ps]), :, row] for x in (other.kp, other.vp))
+            continue
+        k_rows[b], v_rows[b] = kp[c.layer, page, :, row], vp[c.layer, page, :, row]
+        k, v = written[(page, row)]
+        assert_within(k_rows[b], k, pm.EPS[c.dtype] * k.abs() + 2.0 ** -18)
+        assert_within(v_rows[b], v, pm.EPS[c.dtype] * v.abs() + 2.0 ** -21)
+        kp[c.layer, page, :, row], vp[c.layer, page, :, row] = c.kp[c.layer, page, :, row], c.vp[c.layer, page, :, row]
+    bits = torch.int16 if c.dtype == F16 else torch.int32
+    assert torch.equal(kp.view(bits), c.kp.view(bits)) and torch.equal(vp.view(bits), c.vp.view(bits))      # nothing else
+    want, tol = pm.decode(c, ts, k_rows, v_rows, rotary_dim, base, bias)
+    assert_within(out[keep], want[keep], tol[keep])
+    rest = [b for b in range(B) if b not in keep]
+    assert (out[rest] == MARK).all()
+    return out
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("ts,hq,hkv,d,ps", [
+    ([1], 1, 1, 8, 16),
+    ([2, 1, 16, 17], 4, 2, 64, 16),
+    ([33, 64, 65, 129], 7, 1, 128, 64),
+    ([900], 32, 8, 128, 16),
+    ([257, 3000, 1, 511], 8, 8, 128, 32),
+    ([100, 700], 6, 2, 80, 16),
+    ([100, 1300], 16, 1, 96, 256),
+    ([77, 640], 20, 1, 64, 16),
+    ([40, 500], 34, 2, 128, 16),
+    ([90, 1000], 4, 2, 256, 16),
+    ([50, 200], 6, 2, 160, 32),
+])
+def test_decode(capi, dev, dtype, ts, hq, hkv, d, ps):
+    check_decode(capi, decode_case(dtype, ts, hq, hkv, d, ps, seed=31), d)
+
+
+def test_decode_many_sequences_and_layers(capi, dev):
+    ts = [1 + (i * 37) % 400 for i in range(200)]
+    check_decode(capi, decode_case(F16, ts, 8, 2, 64, 16, seed=32, layers=3, layer=1), 64)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_decode_one_long_sequence(capi, dev, dtype):
+    """many pieces per unit; positions far out"""
+    check_decode(capi, decode_case(dtype, [20000], 8, 1, 128, 64, seed=33), 128)
+    check_decode(capi, decode_case(dtype, [30011, 5], 3, 1, 64, 16, seed=34), 64, base=500000.0)
+
+
+def test_decode_partial_rotation_and_no_bias(capi, dev):
+    check_decode(capi, decode_case(F16, [70, 5], 4, 2, 64, 16, seed=35), 32, bias=False)
+    check_decode(capi, decode_case(F32, [70, 5], 4, 2, 64, 16, seed=35), 0)
+    check_decode(capi, decode_case(F16, [70, 5], 4, 2, 64, 16, seed=35), 128)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_decode_lengths_out_of_range_are_left_alone(capi, dev, dtype):
+    c = decode_case(dtype, [40, 100, 7, 90, 33], 4, 2, 64, 16, seed=36)
+    c.ts = [0, 100, -7, 101, 33]
+    c.t_dev = torch.tensor(c.ts, dtype=torch.int32, device=c.q.device)
+    check_decode(capi, c, 64, max_t=100, skip=(0, 2, 3))
+    c.ts = [0, 100, -7, 1000, 33]                            # past the table
+    c.t_dev = torch.tensor(c.ts, dtype=torch.int32, device=c.q.device)
+    check_decode(capi, c, 64, max_t=5000, skip=(0, 2, 3))
+    c.t_dev.fill_(0)
+    c.ts = [0] * 5
+    check_decode(capi, c, 64, max_t=100, skip=range(5))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_decode_rows_without_a_page_take_no_part(capi, dev, dtype):
+    c = decode_case(dtype, [400, 150, 3000, 20], 6, 2, 64, 16, seed=37)
+    for b, p, value in ((0, 0, -1), (0, 7, c.num_pages), (0, 24, -9), (1, 4, 2 ** 31 - 1), (1, 9, -2 ** 31)):
+        c.table[b, p] = value
+    c.table[2, 10:180] = -1                                  # whole pieces without a row
+    c.table[3] = -1                                          # nothing but the new token
+    check_decode(capi, c, 64)
+
+
+def test_decode_workspace_with_and_without_the_flag(capi, dev):
+    cases = [decode_case(F16, [5000, 300], 8, 2, 128, 16, seed=38), decode_case(F32, [1, 900, 4000], 4, 1, 64, 32, seed=39)]
+    size = max(capi.paged_decode_attn_workspace_bytes(len(c.ts), c.hq, c.hkv, c.d, max(c.ts)) for c in cases)
+    ws = torch.zeros(size, dtype=torch.uint8, device=dev)
+    plain = [check_decode(capi, c, c.d) for c in cases]
+    for _ in range(20):                                      # shapes in turn on one zero-filled workspace
+        for c, want in zip(cases, plain):
+            out = run_decode(capi, c, c.kp.clone(), c.vp.clone(), c.d, flags=capi.ATTN_ZEROED_WORKSPACE, workspace=ws)
+            assert torch.equal(out, want)
+    dirty = torch.full((size,), 0x5A, dtype=torch.uint8, device=dev)
+    for c, want in zip(cases, plain):
+        assert torch.equal(run_decode(capi, c, c.kp.clone(), c.vp.clone(), c.d, workspace=dirty), want)
+
+
+def test_decode_on_other_streams_and_in_graphs(capi, dev):
+    cases = [decode_case(F16, [3000, 800], 8, 2, 128, 16, seed=40 + i) for i in range(2)]
+    want = [check_decode(capi, c, 128) for c in cases]
+    outs = [torch.full_like(w, MARK) for w in want]
+    torch.cuda.synchronize()
+    for c, o in zip(cases, outs):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            capi.paged_decode_attn(c.qkv, c.bias, c.kp, c.vp, o, c.table, c.t_dev, 3000, 128, 10000.0)
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
+    # two captured calls share a zero-filled workspace; the lengths grow between replays
+    c = cases[0]
+    ws = torch.zeros(capi.paged_decode_attn_workspace_bytes(2, 8, 2, 128, 3000), dtype=torch.uint8, device=dev)
+    outs = [torch.full_like(want[0], MARK) for _ in range(2)]
+    graphs = []
+    for o in outs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            capi.paged_decode_attn(c.qkv, c.bias, c.kp, c.vp, o, c.table, c.t_dev, 3000, 128, 10000.0,
+                                   flags=capi.ATTN_ZEROED_WORKSPACE, workspace=ws)
+        graphs.append(g)
+    for _ in range(3):
+        for g, o in zip(graphs, outs):
+            o.fill_(MARK)
+            g.replay()
+        torch.cuda.synchronize()
+        for o in outs:
+            assert torch.equal(o, want[0])
+        c.ts = [c.ts[0] - 700, c.ts[1] + 1]
+        c.t_dev.copy_(torch.tensor(c.ts, dtype=torch.int32))
+        want[0] = check_decode(capi, c, 128, max_t=3000)
+
+
+def test_decode_beyond_four_gigabytes(capi, dev):
+    c = decode_case(F16, [150], 4, 2, 128, 16, seed=43)
+    want = check_decode(capi, c, 128)
+    big = 2 ** 32 // (2 * 16 * 128 * 2) * 5 // 4
+    kp, vp = (torch.zeros(1, big, 2, 16, 128, dtype=F16, device=dev) for _ in range(2))
+    near = c.table.clone()
+    for p in range(10):
+        page = big - 1 - 3 * p
+        kp[0, page], vp[0, page] = c.kp[0, int(near[0, p])], c.vp[0, int(near[0, p])]
+        c.table[0, p] = page
+    assert torch.equal(run_decode(capi, c, kp, vp, 128), want)
+
+
+def test_decode_agrees_with_the_contiguous_cache(capi, dev):
+    """the same step on onellm_decode_attn's cache, positions from 0 as prompts write them"""
+    c = decode_case(F16, [700, 700, 700], 8, 2, 128, 16, seed=44)
+    out = check_decode(capi, c, 128)
+    kc = torch.zeros(1, 3, 2, 704, 128, dtype=F16, device=dev)
+    vc = torch.zeros_like(kc)
+    for b in range(3):
+        for p in range(44):
+            kc[0, b, :, 16 * p:16 * p + 16] = c.kp[0, int(c.table[b, p])]
+            vc[0, b, :, 16 * p:16 * p + 16] = c.vp[0, int(c.table[b, p])]
+    flat = torch.empty(3, 8 * 128, dtype=F16, device=dev)
+    capi.decode_attn(c.qkv, c.bias, kc, vc, flat, 8, 700, 128, 10000.0, rope_pos_offset=-1)
+    torch.testing.assert_close(out.view(3, -1), flat, rtol=1e-2, atol=2e-3)

@@ -44,7 +44,17 @@ def prompt(capi, **kw):
                                                a["max_rows"], ptr(a["ws"]), a["ws_bytes"], None)
 
 
-@pytest.mark.parametrize("call", [store, prompt])
+def decode(capi, **kw):
+    a = dict(dtype=1, qkv=FAKE, bias=None, kp=FAKE, vp=FAKE, out=FAKE, table=FAKE, t=FAKE, B=2, Hq=4, Hkv=2, D=128, page=16, num_pages=9,
+             max_pages=4, layer=1, L=2, max_t=64, rot=128, base=10000.0, flags=0, ws=FAKE, ws_bytes=2 ** 40)
+    a.update(kw)
+    return capi.lib().onellm_paged_decode_attn(a["dtype"], ptr(a["qkv"]), ptr(a["bias"]), ptr(a["kp"]), ptr(a["vp"]), ptr(a["out"]),
+                                               ptr(a["table"]), ptr(a["t"]), a["B"], a["Hq"], a["Hkv"], a["D"], a["page"],
+                                               a["num_pages"], a["max_pages"], a["layer"], a["L"], a["max_t"], a["rot"], a["base"],
+                                               a["flags"], ptr(a["ws"]), a["ws_bytes"], None)
+
+
+@pytest.mark.parametrize("call", [store, prompt, decode])
 @pytest.mark.parametrize("kw,code", GEOMETRY_REFUSALS)
 def test_geometry(capi, call, kw, code):
     assert call(capi, **kw) == getattr(capi, code)
@@ -72,6 +82,19 @@ def test_store_refusals(capi, kw, code):
 ])
 def test_prompt_refusals(capi, kw, code):
     assert prompt(capi, **kw) == getattr(capi, code)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(qkv=None), "EINVAL"), (dict(out=None), "EINVAL"), (dict(t=None), "EINVAL"), (dict(max_t=0), "EINVAL"), (dict(max_t=-4), "EINVAL"),
+    (dict(flags=1), "EINVAL"), (dict(flags=2), "EINVAL"), (dict(flags=12), "EINVAL"), (dict(rot=-2), "EINVAL"), (dict(rot=7), "EINVAL"),
+    (dict(base=0.0), "EINVAL"), (dict(base=float("nan")), "EINVAL"),
+    (dict(qkv=FAKE + 4), "EUNSUPPORTED"), (dict(out=FAKE + 8), "EUNSUPPORTED"), (dict(bias=FAKE + 2), "EUNSUPPORTED"),
+    (dict(ws=None), "EWORKSPACE"), (dict(ws=FAKE + 4), "EWORKSPACE"), (dict(ws_bytes=4096), "EWORKSPACE"),
+    # more work than the schedule can number, however coarse its items
+    (dict(B=65535, Hq=4096, Hkv=4096, max_t=64), "EUNSUPPORTED"),
+])
+def test_decode_refusals(capi, kw, code):
+    assert decode(capi, **kw) == getattr(capi, code)
 
 
 def test_no_tokens_is_no_work(capi):
