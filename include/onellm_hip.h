@@ -350,6 +350,25 @@ int onellm_paged_decode_attn(int dtype, const void* qkv, const void* qkv_bias, v
                              void* workspace, size_t workspace_bytes, onellm_stream_t stream);
 size_t onellm_paged_decode_attn_workspace_bytes(int B, int Hq, int Hkv, int D, int max_t);
 
+/*
+ * Log-probabilities of given tokens, entropy and the K likeliest tokens of N rows of logits: what a service answers with beside a
+ * token, or scores a prompt by.  No counterpart in the reference, whose sampling keeps no probabilities
+ * (src/kernels/topK_sampling.cu:6-70).  With lse = log sum_v exp(x_v):
+ *   logprob[n] = x[n, targets[n]] - lse   (0 where targets[n] lies outside [0, V): no token to score)
+ *   entropy[n] = lse - sum_v p_v x_v,  p_v = exp(x_v - lse)
+ *   top_ids, top_logprobs [N, K]: the K largest logits, larger value first, equal values: smaller token first, and x - lse
+ * logits: row n at logits + n * ld elements (ld >= V), fp16 or fp32, any alignment; targets device int32[N]; outputs fp32 / int32.
+ * logprob (with targets), entropy may be NULL, K may be 0 (then top_ids, top_logprobs are not read); 0 <= K <= 32, V <= 2^28,
+ * N <= 2^26.
+ * A logit of -inf (a banned token) has no probability and is never among the top; slots left over hold id -1 and -inf.  A row
+ * of nothing but -inf: logprob -inf, entropy 0.  A NaN or +inf logit makes the row's logprob and entropy NaN; NaNs are never among the top.
+ * workspace: onellm_token_logprobs_workspace_bytes() bytes, 16-byte aligned, contents irrelevant; calls that share one must not overlap.
+ */
+int onellm_token_logprobs(int dtype, const void* logits, long ld, const int* targets, int N, int V, int K,
+                          float* logprob, float* entropy, int* top_ids, float* top_logprobs,
+                          void* workspace, size_t workspace_bytes, onellm_stream_t stream);
+size_t onellm_token_logprobs_workspace_bytes(int N, int V, int K);
+
 #ifdef __cplusplus
 }
 #endif

@@ -38,7 +38,8 @@ DRIVER_SRC = os.path.join(ROOT, "tests", "cpp", "self_decoder_driver.cpp")
 DRIVER_BIN = os.path.join(ROOT, "tests", "cpp", "self_decoder_driver")
 
 KERNEL_SOURCES = ["decode_attn.hip", "norms.hip", "kv_cache.hip", "beam_topk.hip", "prefill_rope.hip", "activation.hip", "sampling.hip",
-                  "paged_store.hip", "paged_prompt.hip", "paged_decode.hip", "tuning.cpp", "counter_sets.cpp"]
+                  "paged_store.hip", "paged_prompt.hip", "paged_decode.hip", "logprobs.hip",
+                  "tuning.cpp", "counter_sets.cpp"]
 LAUNCHER_SOURCES = ["launchers.cpp"]
 GEMM_SOURCES = ["linear.hip", "skinny_gemm.hip"]
 LAYER_SOURCES = ["layers.cpp", "layers_capi.cpp"]

@@ -50,6 +50,8 @@ SYMBOLS = {
     "onellm_paged_prompt_attn": (_ci, [_ci, _vp, _cl, _vp, _vp, _vp, _cl, _vp, _vp, _vp] + [_ci] * 11 + [_vp, _sz, _vp]),
     "onellm_paged_decode_attn": (_ci, [_ci] + [_vp] * 7 + [_ci] * 11 + [_cf, _cu, _vp, _sz, _vp]),
     "onellm_paged_decode_attn_workspace_bytes": (_sz, [_ci, _ci, _ci, _ci, _ci]),
+    "onellm_token_logprobs": (_ci, [_ci, _vp, _cl, _vp, _ci, _ci, _ci, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "onellm_token_logprobs_workspace_bytes": (_sz, [_ci, _ci, _ci]),
     "onellm_paged_prompt_attn_workspace_bytes": (_sz, [_ci, _ci, _ci, _ci, _ci, _ci]),
 }
 
@@ -367,6 +369,34 @@ def paged_decode_attn(qkv, bias, k_pages, v_pages, out, block_table, t_dev, max_
                                           block_table.shape[1], layer, L, int(max_t), rotary_dim, rope_base, flags,
                                           _ptr(workspace), workspace.numel(), _stream()), "onellm_paged_decode_attn")
     return out
+
+
+def token_logprobs_workspace_bytes(N, V, K):
+    return lib().onellm_token_logprobs_workspace_bytes(N, V, K)
+
+
+def token_logprobs(logits, targets, K, logprob, entropy, top_ids, top_logprobs, workspace=None):
+    """logits [N, V], rows may be a stride apart; targets int32 [N]; logprob, entropy fp32 [N] (either may be None); top_ids int32
+    and top_logprobs fp32 [N, K] (unused when K is 0).  `workspace`: uint8 device tensor; allocated here when None."""
+    import torch
+    N, V = logits.shape
+    if logits.stride(1) != 1 and V > 1:
+        raise ValueError("logits [N, V] with contiguous rows expected")
+    for t, shape in ((logprob, (N,)), (entropy, (N,)), (top_logprobs if K else None, (N, K))):
+        if t is not None and (t.shape != shape or t.dtype != torch.float32):
+            raise ValueError(f"fp32 output of shape {shape} expected")
+    if K and top_ids.shape != (N, K) or targets is not None and targets.numel() != N:
+        raise ValueError("top_ids [N, K] and targets [N] expected")
+    if workspace is None:
+        workspace = torch.empty(token_logprobs_workspace_bytes(N, V, K), dtype=torch.uint8, device=logits.device)
+    if not K:
+        top_ids = top_logprobs = None
+    _same_device(logits, targets, logprob, entropy, top_ids, top_logprobs, workspace)
+    _int32(targets, top_ids)
+    _check(lib().onellm_token_logprobs(_dt(logits), logits.data_ptr(), logits.stride(0) if N > 1 else max(V, logits.stride(0)),
+                                       _ptr(targets), N, V, K, _ptr(logprob), _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs),
+                                       _ptr(workspace), workspace.numel(), _stream()), "onellm_token_logprobs")
+    return logprob, entropy, top_ids, top_logprobs
 
 
 # ---------------------------------------------------------------- projection GEMMs (include/onellm_gemm.h)

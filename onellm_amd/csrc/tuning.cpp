@@ -46,7 +46,7 @@ int tune_get(const char* key)
 // 1.1: ONELLM_ATTN_ZEROED_WORKSPACE, 64 KiB of arrival counters at the front of the attention workspace
 // 1.2: onellm_decode_attn_static
 // 1.3: onellm_release_workspace, onellm_counter_set_fallbacks, onellm_beam_topk_last_path
-// 1.4: the paged key-value cache: onellm_paged_qkv_store, onellm_paged_prompt_attn, onellm_paged_decode_attn
+// 1.4: the paged key-value cache: onellm_paged_qkv_store, onellm_paged_prompt_attn, onellm_paged_decode_attn; onellm_token_logprobs
 extern "C" int onellm_hip_version(void) { return 1004; }
 
 extern "C" int onellm_tune_set(const char* key, int value)

@@ -97,7 +97,26 @@ def test_decode_refusals(capi, kw, code):
     assert decode(capi, **kw) == getattr(capi, code)
 
 
+def logprobs(capi, **kw):
+    a = dict(dtype=1, x=FAKE, ld=100000, targets=FAKE, N=3, V=100000, K=5, lp=FAKE, ent=FAKE, ids=FAKE, tops=FAKE, ws=FAKE, ws_bytes=2 ** 40)
+    a.update(kw)
+    return capi.lib().onellm_token_logprobs(a["dtype"], ptr(a["x"]), a["ld"], ptr(a["targets"]), a["N"], a["V"], a["K"], ptr(a["lp"]),
+                                            ptr(a["ent"]), ptr(a["ids"]), ptr(a["tops"]), ptr(a["ws"]), a["ws_bytes"], None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dtype=2), "EINVAL"), (dict(x=None), "EINVAL"), (dict(x=FAKE + 1), "EINVAL"), (dict(dtype=0, x=FAKE + 2), "EINVAL"),
+    (dict(targets=None), "EINVAL"), (dict(N=-1), "EINVAL"), (dict(V=0), "EINVAL"), (dict(ld=99999), "EINVAL"), (dict(K=-1), "EINVAL"),
+    (dict(ids=None), "EINVAL"), (dict(tops=None), "EINVAL"), (dict(lp=None, ent=None, K=0), "EINVAL"),
+    (dict(K=33), "EUNSUPPORTED"), (dict(V=2 ** 28 + 1, ld=2 ** 29), "EUNSUPPORTED"), (dict(N=2 ** 26 + 1), "EUNSUPPORTED"),
+    (dict(ws=None), "EWORKSPACE"), (dict(ws=FAKE + 8), "EWORKSPACE"), (dict(ws_bytes=200), "EWORKSPACE"),
+])
+def test_logprobs_refusals(capi, kw, code):
+    assert logprobs(capi, **kw) == getattr(capi, code)
+
+
 def test_no_tokens_is_no_work(capi):
+    assert logprobs(capi, N=0, x=None, targets=None, ids=None, tops=None, ws=None, ws_bytes=0) == 0
     assert store(capi, tokens=0, q_out=None, qkv=None) == 0
     assert prompt(capi, tokens=0, q=None, out=None, ws=None, ws_bytes=0) == 0
 
