@@ -12,6 +12,7 @@
 // keys) comes out of the LDS transposed (ds_read_b64_tr_b16); for fp32 a product takes two keys and reads them as they are.
 // Scores, statistics and output are fp32.  fp16: P enters its product rounded to fp16 (half a step, 2^-12 relative of each
 // weight, averaged over the keys); the sum of the weights is taken before that rounding.
+#include <type_traits>
 #include "paged.hpp"
 
 namespace onellm {
@@ -139,7 +140,7 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
     constexpr int VEC = S::VEC, BN = S::BN, P = S::P, LD = S::LD, NS = S::NS, ND = S::ND;
     // (four arrays, not one: the compiler then sees that the rows on their way to one pair do not touch the other)
     __shared__ __align__(16) char k_even[S::TILE], v_even[S::TILE], k_odd[S::TILE], v_odd[S::TILE];
-    __shared__ unsigned s_bad[3][2];                // keys of a masked step whose V row holds a NaN or an infinity
+    __shared__ int s_odd;                           // a masked step met a NaN or an infinity in V
 
     Tile t;
     if (!locate_tile(a, blockIdx.y, t)) return;
@@ -178,8 +179,9 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
         }
     }
 
-    if (tid < 6) s_bad[tid / 2][tid % 2] = 0;
-    float mx = -INFINITY, l = 0.f;                  // of this lane's row; l over the keys this lane holds
+    if (tid == 0) s_odd = 0;
+    float mx = -INFINITY, l = 0.f;                  // of this lane's row: what weights are relative to; their sum over this lane's keys
+    const float slack = 8.f / a.score_scale;
     f32x16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -204,10 +206,20 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
     // gets piece p' ^ swizzle(row).  A wave's slots lie in one group of 16 rows, which is read through a window that holds
     // the rows the sequence has there: rows behind its end, rows on a page that is none, and pieces behind the head's
     // end arrive as zeros.
+    constexpr int RI = kThreads / P;                // rows between two slots of a thread
+    constexpr int NOFF = RI % kRowGroup == 0 ? 1 : kRowGroup / RI;      // different places inside a window
+    unsigned koff[NOFF], voff[NOFF];
+#pragma unroll
+    for (int i = 0; i < NOFF; ++i) {
+        const int row = i * RI + tid / P, p = tid % P;
+        const unsigned line = (unsigned)((row % kRowGroup) * D) * (unsigned)sizeof(T);
+        const int pk = p ^ S::swz_k(row), pv = p ^ S::swz_v(row);
+        koff[i] = pk * VEC < D ? line + pk * 16 : kOutside;
+        voff[i] = pv * VEC < D ? line + pv * 16 : kOutside;
+    }
     auto request = [&](char* kb, char* vb, int k0) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
-            const int row = (i * kThreads + tid) / P, p = (i * kThreads + tid) % P;
             const int g0 = (i * kThreads + wave * 64) / P / kRowGroup;       // (the wave's group)
             int page = pages.x;
             if constexpr (S::NG > 1) page = g0 == 1 ? pages.y : page;
@@ -218,67 +230,105 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
             const int bytes = rows * D * (int)sizeof(T);
             T* kp = const_cast<T*>(static_cast<const T*>(a.k_pages)) + at;
             T* vp = const_cast<T*>(static_cast<const T*>(a.v_pages)) + at;
-            const unsigned line = (unsigned)((row % kRowGroup) * D) * (unsigned)sizeof(T);
-            const int pk = p ^ S::swz_k(row), pv = p ^ S::swz_v(row);
             typedef __attribute__((address_space(3))) void lds_void;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(kp, 0, bytes, 0x00020000),
-                                                     (lds_void*)(kb + (i * kThreads + wave * 64) * 16), 16,
-                                                     pk * VEC < D ? line + pk * 16 : kOutside, 0, 0, 0);
+                                                     (lds_void*)(kb + (i * kThreads + wave * 64) * 16), 16, koff[i % NOFF], 0, 0, 0);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(vp, 0, bytes, 0x00020000),
-                                                     (lds_void*)(vb + (i * kThreads + wave * 64) * 16), 16,
-                                                     pv * VEC < D ? line + pv * 16 : kOutside, 0, 0, 0);
+                                                     (lds_void*)(vb + (i * kThreads + wave * 64) * 16), 16, voff[i % NOFF], 0, 0, 0);
         }
     };
     // Masked steps: a NaN or an infinity in a V row would reach rows that do not see it (0 * NaN), so every thread
-    // replaces those among the pieces it brought by zeros and notes their keys; compute() adds them to the rows that do see them.
-    auto clean = [&](char* vb, int slot) __attribute__((always_inline)) {
+    // first replaces those among the pieces it brought by zeros; the rows that do see them get them behind the loop.
+    auto clean = [&](char* vb) __attribute__((always_inline)) {
 #pragma unroll 1
         for (int i = 0; i < LD; ++i) {
             Vec16<T>* at = reinterpret_cast<Vec16<T>*>(vb + (i * kThreads + tid) * 16);
             Vec16<T> v = *at;
-            bool bad = false;
+            bool odd = false;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const bool fin = __builtin_fabsf(v.get(e)) < INFINITY;
-                bad = bad || !fin;
+                odd = odd || !fin;
                 v.set(e, fin ? v.get(e) : 0.f);
             }
-            if (bad) {
+            if (odd) {
                 *at = v;
-                const int row = (i * kThreads + tid) / P;
-                atomicOr(&s_bad[slot][row / 32], 1u << (row % 32));
+                s_odd = 1;
             }
         }
     };
 
     // one step: keys k0 .. k0 + BN - 1.  valid: bit g = group g's page exists (masked steps only)
-    auto compute = [&](const char* kb, const char* vb, int k0, auto masked_tag, unsigned valid, int slot) __attribute__((always_inline)) {
+    auto compute = [&](const char* kb, const char* vb, int k0, auto masked_tag, unsigned valid) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked_tag)::value;
+        // Reads from LDS are issued two products ahead (K) or one group of products ahead (V); the scheduling barriers keep
+        // them there - left alone, the compiler reads every operand right before its product and waits for it.
         f32x16 s[NS];
+        Vec16<T> kf[P / 2][NS];
+        auto read_k = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
+            for (int n = 0; n < NS; ++n) {
+                const int row = n * 32 + col;
+                kf[k][n].raw = *reinterpret_cast<const decltype(kf[k][n].raw)*>(kb + row * S::ROW + ((2 * k + half) ^ S::swz_k(row)) * 16);
+            }
+        };
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
-            const int row = n * 32 + col;
+        read_k(0);
+        read_k(1);
 #pragma unroll
-            for (int k = 0; k < P / 2; ++k) {
-                Vec16<T> kf;
-                kf.raw = *reinterpret_cast<const decltype(kf.raw)*>(kb + row * S::ROW + ((2 * k + half) ^ S::swz_k(row)) * 16);
+        for (int k = 0; k < P / 2; ++k) {
+            if (k + 2 < P / 2) read_k(k + 2);
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
                 if constexpr (S::kHalf) {
-                    s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf.raw, qf[k].raw, s[n], 0, 0, 0);
+                    s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k][n].raw, qf[k].raw, s[n], 0, 0, 0);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.raw[e], qf[k].raw[e], s[n], 0, 0, 0);
+                    for (int e = 0; e < 4; ++e) s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[k][n].raw[e], qf[k].raw[e], s[n], 0, 0, 0);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
+        // V^T operands.  fp16: of 16 keys, 16 i + 8 (e / 4) + 4 half + e % 4, which is what the score registers 8 (i % 2) .. + 7
+        // of this lane are: 16 lanes read four rows x 16 columns, four elements each, and get one column of the four rows each.
+        // fp32: of the two keys (one per half) that score register i is.
+        constexpr int GROUPS = S::kHalf ? BN / 16 : NS * 16;
+        using VFrag = typename std::conditional<S::kHalf, f16x8, float>::type;
+        VFrag vf[GROUPS][ND];
+        auto read_v = [&](int i) __attribute__((always_inline)) {
+            if constexpr (S::kHalf) {
+                const int row = 16 * i + 4 * half + (lane & 15) / 4, row2 = row + 8;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const int piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4*)(vb + row * S::ROW + (piece ^ S::swz_v(row)) * 16 + (lane & 1) * 8));
+                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4*)(vb + row2 * S::ROW + (piece ^ S::swz_v(row2)) * 16 + (lane & 1) * 8));
+                    vf[i][d] = __builtin_bit_cast(f16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+            } else {
+                const int row = (i / 16) * 32 + 8 * (i % 16 / 4) + 4 * half + i % 4;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const int piece = 8 * d + col / 4;
+                    vf[i][d] = *reinterpret_cast<const float*>(vb + row * S::ROW + (piece ^ S::swz_v(row)) * 16 + (col % 4) * 4);
+                }
+            }
+        };
+        read_v(0);
+        __builtin_amdgcn_sched_barrier(0);
         if constexpr (MASKED) {
+            const int room = limit - k0 - 4 * half;
 #pragma unroll
             for (int n = 0; n < NS; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int key = n * 32 + 8 * (r / 4) + 4 * half + r % 4;
-                    const bool see = k0 + key <= limit && (valid >> (n * 2 + r / 8) & 1u);
+                    const bool see = n * 32 + 8 * (r / 4) + r % 4 <= room && (valid >> (n * 2 + r / 8) & 1u);
                     s[n][r] = see ? s[n][r] : -INFINITY;
                 }
         }
@@ -288,7 +338,9 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
 #pragma unroll
             for (int r = 0; r < 16; ++r) bm = fmaxf(bm, s[n][r]);
         bm = other_half_max(bm);
-        if (__builtin_amdgcn_ballot_w64(bm > mx) != 0) {
+        // What the weights are taken against only follows the maximum when that has grown by 2^8 or more: weights of up to 256 lose
+        // nothing (a rounding is relative), and a row's sum and output are rescaled a few times, not every few steps.
+        if (__builtin_amdgcn_ballot_w64(bm > mx + slack) != 0) {
             const float mnew = fmaxf(mx, bm);
             const float alpha = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mx - mnew) * a.score_scale);
             l *= alpha;
@@ -306,116 +358,105 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
                 s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.score_scale, -shift));
                 l += s[n][r];
             }
-        if constexpr (S::kHalf) {
 #pragma unroll
-            for (int i = 0; i < BN / 16; ++i) {
-                // keys 16 i + 8 (e / 4) + 4 half + e % 4: what the score registers 8 (i % 2) .. + 7 of this lane are
+        for (int i = 0; i < GROUPS; ++i) {
+            if (i + 1 < GROUPS) read_v(i + 1);
+            if constexpr (S::kHalf) {
                 f16x8 pf;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) pf[e] = (_Float16)s[i / 2][8 * (i % 2) + e];
-                // 16 lanes read four rows x 16 columns, four elements each, and get one column of the four rows each
-                const int row = 16 * i + 4 * half + (lane & 15) / 4;
-                const int row2 = row + 8;
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    const int piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s16x4*)(vb + row * S::ROW + (piece ^ S::swz_v(row)) * 16 + (lane & 1) * 8));
-                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s16x4*)(vb + row2 * S::ROW + (piece ^ S::swz_v(row2)) * 16 + (lane & 1) * 8));
-                    const f16x8 vf = __builtin_bit_cast(f16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf, o[d], 0, 0, 0);
-                }
+                for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i][d], pf, o[d], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[i][d], s[i / 16][i % 16], o[d], 0, 0, 0);
             }
-        } else {
-#pragma unroll
-            for (int n = 0; n < NS; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int row = n * 32 + 8 * (r / 4) + 4 * half + r % 4;
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        const int piece = 8 * d + col / 4;
-                        const float vf = *reinterpret_cast<const float*>(vb + row * S::ROW + (piece ^ S::swz_v(row)) * 16 + (col % 4) * 4);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[n][r], o[d], 0, 0, 0);
-                    }
-                }
-        }
-        if constexpr (MASKED) {
-            // (rare) keys with a NaN or an infinity in V: added to the rows that see them.  A weight of any size times
-            // such a value is that value.
-#pragma unroll 1
-            for (int w = 0; w < (BN + 31) / 32; ++w) {
-                unsigned bits = __builtin_amdgcn_readfirstlane(s_bad[slot][w]);
-#pragma unroll 1
-                while (bits) {
-                    const int key = k0 + w * 32 + __builtin_ctz(bits);
-                    bits &= bits - 1;
-                    const int page = __builtin_amdgcn_readfirstlane(page_of(a.cache, table, key));
-                    if (page < 0) continue;
-                    const T* v = static_cast<const T*>(a.v_pages) + paged_offset(a.cache, page, kvh, key);
-                    const __amdgpu_buffer_rsrc_t w = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(v), 0, D * (int)sizeof(T), 0x00020000);
-                    const bool see = key <= limit;
-#pragma unroll
-                    for (int d = 0; d < ND; ++d)
-#pragma unroll
-                        for (int r4 = 0; r4 < 4; ++r4) {
-                            const Quad<T> x = load_quad<T>(w, (32 * d + 8 * r4 + 4 * half) * (int)sizeof(T));
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float f = to_f32(x.v[e]);
-                                o[d][4 * r4 + e] += see && !(__builtin_fabsf(f) < INFINITY) ? f : 0.f;
-                            }
-                            __builtin_amdgcn_sched_barrier(0);       // (four values at a time: no registers for a path this rare)
-                        }
-                }
-            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
     if (k_begin < k_end) {
+        // Steps that every row of the tile sees whole, and whose pages all exist, go in pairs (a buffer pair each) with nothing
+        // conditional in between; the rest - the diagonal, as a rule - are masked.
         const int steps = (k_end - k_begin + BN - 1) / BN;
-        const int plain = max(0, min(k_end, rows_all) - k_begin) / BN;     // steps that every row of the tile sees whole
+        const int plain = max(0, min(k_end, rows_all) - k_begin) / BN;
         constexpr unsigned kAll = (1u << S::NG) - 1u;
-        unsigned valid = 0;
-        bool masked = false;
-        int it = 0;
-        auto look = [&](int step) __attribute__((always_inline)) {                 // what the pages of a step say about it
-            valid = (pages.x >= 0 ? 1u : 0u) | (pages.y >= 0 ? 2u : 0u);
-            if constexpr (S::NG > 2) valid |= (pages.z >= 0 ? 4u : 0u) | (pages.w >= 0 ? 8u : 0u);
-            masked = step >= plain || valid != kAll;
+        auto valid_of = [&]() __attribute__((always_inline)) {
+            unsigned v = (pages.x >= 0 ? 1u : 0u) | (pages.y >= 0 ? 2u : 0u);
+            if constexpr (S::NG > 2) v |= (pages.z >= 0 ? 4u : 0u) | (pages.w >= 0 ? 8u : 0u);
+            return v;
         };
-        auto arrive = [&](char* vb, int slot) __attribute__((always_inline)) {     // this wave's rows are there; then everybody's
+        auto arrive = [&]() __attribute__((always_inline)) {               // this wave's rows are there; then everybody's
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (masked) clean(vb, slot);
             __syncthreads();
         };
-        auto step = [&](char* kb, char* vb, char* kn, char* vn) __attribute__((always_inline)) {
-            const int k0 = k_begin + it * BN;
-            const unsigned valid_now = valid;
-            const bool masked_now = masked, more = it + 1 < steps;
-            if (more) {
-                request(kn, vn, k0 + BN);
-                look(it + 1);
-                fetch_pages(k0 + 2 * BN);
-            }
-            if (masked_now) compute(kb, vb, k0, std::true_type{}, valid_now, it % 3);
-            else compute(kb, vb, k0, std::false_type{}, kAll, 0);
-            if (more) {
-                if (tid < 2) s_bad[(it + 2) % 3][tid] = 0;       // (last read before the previous barrier, next written behind the coming one)
-                arrive(vn, (it + 1) % 3);
-            }
+        int it = 0, k0 = k_begin;
+        unsigned valid;                                                  // of step `it`; `pages` are those of step it + 1
+        // (rows behind the last step are requested like the others: their windows are empty)
+        auto next = [&](char* kn, char* vn) __attribute__((always_inline)) {
+            request(kn, vn, k0 + BN);
+            valid = valid_of();
+            fetch_pages(k0 + 2 * BN);
+        };
+        auto plain_step = [&](char* kb, char* vb, char* kn, char* vn) __attribute__((always_inline)) {
+            next(kn, vn);
+            compute(kb, vb, k0, std::false_type{}, kAll);
+            arrive();
             ++it;
-            return more;
+            k0 += BN;
+        };
+        auto masked_step = [&](char* kb, char* vb, char* kn, char* vn) __attribute__((always_inline)) {
+            const unsigned now = valid;
+            clean(vb);
+            __syncthreads();
+            next(kn, vn);
+            compute(kb, vb, k0, std::true_type{}, now);
+            arrive();
+            ++it;
+            k0 += BN;
         };
         fetch_pages(k_begin);
         request(k_even, v_even, k_begin);
-        look(0);
+        valid = valid_of();
         fetch_pages(k_begin + BN);
-        __syncthreads();                                         // s_bad is clear
-        arrive(v_even, 0);
-        while (step(k_even, v_even, k_odd, v_odd) && step(k_odd, v_odd, k_even, v_even)) {}
+        arrive();
+        while (it + 2 <= plain && (valid & valid_of()) == kAll) {
+            plain_step(k_even, v_even, k_odd, v_odd);
+            plain_step(k_odd, v_odd, k_even, v_even);
+        }
+        const int odd_from = k0;                                         // first key of the masked steps
+        while (it < steps) {
+            masked_step(k_even, v_even, k_odd, v_odd);
+            if (it >= steps) break;
+            masked_step(k_odd, v_odd, k_even, v_even);
+        }
+
+        // (rare) NaNs and infinities in V rows of masked steps reach the rows that see them: a weight of any size times such a
+        // value is that value.
+        if (__builtin_amdgcn_readfirstlane(s_odd)) {
+#pragma unroll 1
+            for (int key = odd_from; key < k_end; ++key) {
+                const int page = __builtin_amdgcn_readfirstlane(page_of(a.cache, table, key));
+                if (page < 0) continue;
+                const T* v = static_cast<const T*>(a.v_pages) + paged_offset(a.cache, page, kvh, key);
+                const __amdgpu_buffer_rsrc_t w = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(v), 0, D * (int)sizeof(T), 0x00020000);
+                const bool see = key <= limit;
+                int at = 4 * half * (int)sizeof(T);
+                asm volatile("" : "+v"(at));                   // (offsets made here, not held in registers across the steps)
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; ++r4) {
+                        const Quad<T> x = load_quad<T>(w, at + (32 * d + 8 * r4) * (int)sizeof(T));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float f = to_f32(x.v[e]);
+                            o[d][4 * r4 + e] += see && !(__builtin_fabsf(f) < INFINITY) ? f : 0.f;
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            }
+        }
     }
 
     l += __shfl_xor(l, 32, kWave);
