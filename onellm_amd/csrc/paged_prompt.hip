@@ -188,19 +188,22 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
 
-    typedef int Pages __attribute__((ext_vector_type(4)));
-    Pages pages = {0, 0, 0, 0};                     // of the row groups of the step that is requested next
-    static_assert(S::NG <= 4, "row groups per step");
-    auto fetch_pages = [&](int k0) __attribute__((always_inline)) {
-        auto one = [&](int row) __attribute__((always_inline)) {
-            return row < k_end ? __builtin_amdgcn_readfirstlane(page_of(a.cache, table, row)) : 0;
-        };
-        pages.x = one(k0);
-        pages.y = one(k0 + kRowGroup);
-        if constexpr (S::NG > 2) {
-            pages.z = one(k0 + 2 * kRowGroup);
-            pages.w = one(k0 + 3 * kRowGroup);
-        }
+    // Where the rows are.  A step's rows are NG groups of 16 and every wave needs each group's address in scalar registers; looked
+    // up one by one that was 240 scalar instructions per step, a third of the kernel's time.  So the lanes of a wave look
+    // up 64 groups at once - lane g the g-th of a block of SPB steps - and a step reads its groups' offsets out of them.
+    constexpr int SPB = kWave / S::NG;              // steps per block
+    auto pages_of = [&](int block) __attribute__((always_inline)) {      // page of this lane's group, -1: none
+        const int row = k_begin + (block * kWave + lane) * kRowGroup;
+        const int id = table[min(row, k_end - 1) >> a.cache.page_shift];     // (k_end lies inside the table; no branch around the load)
+        return row < k_end && (unsigned)id < (unsigned)a.cache.num_pages ? id : -1;
+    };
+    unsigned off_lo = 0, off_hi = 0;                // byte offset of this lane's group in the page arrays
+    unsigned long long there = 0;                   // the groups of the block that have a page
+    auto open_block = [&](int block, int page) __attribute__((always_inline)) {
+        there = __builtin_amdgcn_ballot_w64(page >= 0);
+        const size_t at = paged_offset(a.cache, max(page, 0), kvh, k_begin + (block * kWave + lane) * kRowGroup) * sizeof(T);
+        off_lo = (unsigned)at;
+        off_hi = (unsigned)(at >> 32);
     };
     // Rows k0 .. k0 + BN - 1 go straight from memory to LDS, 16 bytes per lane: slot (tid + 256 i) is (row, p') and
     // gets piece p' ^ swizzle(row).  A wave's slots lie in one group of 16 rows, which is read through a window that holds
@@ -217,19 +220,20 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
         koff[i] = pk * VEC < D ? line + pk * 16 : kOutside;
         voff[i] = pv * VEC < D ? line + pv * 16 : kOutside;
     }
-    auto request = [&](char* kb, char* vb, int k0) __attribute__((always_inline)) {
+    // EDGE: the step may reach past the sequence's end or lie on pages that are none (without it the rows are all there,
+    // or stand on a page that is not looked at: a masked step leaves them out)
+    auto request = [&](char* kb, char* vb, int step, auto edge_tag) __attribute__((always_inline)) {
+        constexpr bool EDGE = decltype(edge_tag)::value;
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
-            const int g0 = (i * kThreads + wave * 64) / P / kRowGroup;       // (the wave's group)
-            int page = pages.x;
-            if constexpr (S::NG > 1) page = g0 == 1 ? pages.y : page;
-            if constexpr (S::NG > 2) page = g0 == 2 ? pages.z : (g0 == 3 ? pages.w : page);
-            const int row0 = k0 + g0 * kRowGroup;
-            const int rows = page < 0 ? 0 : rows_left(k_end, row0);
-            const size_t at = paged_offset(a.cache, max(page, 0), kvh, row0);
+            const int group = step * S::NG + (i * kThreads + wave * 64) / P / kRowGroup;       // (the wave's group)
+            const size_t at = (size_t)(unsigned)__builtin_amdgcn_readlane((int)off_hi, group % kWave) << 32
+                              | (unsigned)__builtin_amdgcn_readlane((int)off_lo, group % kWave);
+            int rows = kRowGroup;
+            if constexpr (EDGE) rows = (there >> (group % kWave) & 1) ? rows_left(k_end, k_begin + group * kRowGroup) : 0;
             const int bytes = rows * D * (int)sizeof(T);
-            T* kp = const_cast<T*>(static_cast<const T*>(a.k_pages)) + at;
-            T* vp = const_cast<T*>(static_cast<const T*>(a.v_pages)) + at;
+            char* kp = const_cast<char*>(static_cast<const char*>(a.k_pages)) + at;
+            char* vp = const_cast<char*>(static_cast<const char*>(a.v_pages)) + at;
             typedef __attribute__((address_space(3))) void lds_void;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(kp, 0, bytes, 0x00020000),
                                                      (lds_void*)(kb + (i * kThreads + wave * 64) * 16), 16, koff[i % NOFF], 0, 0, 0);
@@ -380,49 +384,43 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
         // conditional in between; the rest - the diagonal, as a rule - are masked.
         const int steps = (k_end - k_begin + BN - 1) / BN;
         const int plain = max(0, min(k_end, rows_all) - k_begin) / BN;
-        constexpr unsigned kAll = (1u << S::NG) - 1u;
-        auto valid_of = [&]() __attribute__((always_inline)) {
-            unsigned v = (pages.x >= 0 ? 1u : 0u) | (pages.y >= 0 ? 2u : 0u);
-            if constexpr (S::NG > 2) v |= (pages.z >= 0 ? 4u : 0u) | (pages.w >= 0 ? 8u : 0u);
-            return v;
-        };
+        constexpr unsigned kAll = (1u << S::NG) - 1u, kPair = (1u << 2 * S::NG) - 1u;
+        auto there_from = [&](int step) __attribute__((always_inline)) { return (unsigned)(there >> (step * S::NG % kWave)); };
         auto arrive = [&]() __attribute__((always_inline)) {               // this wave's rows are there; then everybody's
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
         };
-        int it = 0, k0 = k_begin;
-        unsigned valid;                                                  // of step `it`; `pages` are those of step it + 1
+        int it = 0, k0 = k_begin, page = 0;
         // (rows behind the last step are requested like the others: their windows are empty)
-        auto next = [&](char* kn, char* vn) __attribute__((always_inline)) {
-            request(kn, vn, k0 + BN);
-            valid = valid_of();
-            fetch_pages(k0 + 2 * BN);
+        auto next = [&](char* kn, char* vn, auto edge_tag) __attribute__((always_inline)) {
+            const int step = it + 1;
+            if (step % SPB == 0) open_block(step / SPB, page);
+            page = pages_of(step / SPB + 1);        // the next block's: asked for in every step, a branch more costs more
+            request(kn, vn, step, edge_tag);
         };
-        auto plain_step = [&](char* kb, char* vb, char* kn, char* vn) __attribute__((always_inline)) {
-            next(kn, vn);
+        auto plain_step = [&](char* kb, char* vb, char* kn, char* vn, auto edge_tag) __attribute__((always_inline)) {
+            next(kn, vn, edge_tag);
             compute(kb, vb, k0, std::false_type{}, kAll);
             arrive();
             ++it;
             k0 += BN;
         };
         auto masked_step = [&](char* kb, char* vb, char* kn, char* vn) __attribute__((always_inline)) {
-            const unsigned now = valid;
+            const unsigned now = there_from(it) & kAll;
             clean(vb);
             __syncthreads();
-            next(kn, vn);
+            next(kn, vn, std::true_type{});
             compute(kb, vb, k0, std::true_type{}, now);
             arrive();
             ++it;
             k0 += BN;
         };
-        fetch_pages(k_begin);
-        request(k_even, v_even, k_begin);
-        valid = valid_of();
-        fetch_pages(k_begin + BN);
+        open_block(0, pages_of(0));
+        request(k_even, v_even, 0, std::true_type{});
         arrive();
-        while (it + 2 <= plain && (valid & valid_of()) == kAll) {
-            plain_step(k_even, v_even, k_odd, v_odd);
-            plain_step(k_odd, v_odd, k_even, v_even);
+        while (it + 2 <= plain && (there_from(it) & kPair) == kPair) {      // (a pair lies in one block)
+            plain_step(k_even, v_even, k_odd, v_odd, std::false_type{});
+            plain_step(k_odd, v_odd, k_even, v_even, std::true_type{});
         }
         const int odd_from = k0;                                         // first key of the masked steps
         while (it < steps) {
