@@ -36,56 +36,58 @@ struct PromptArgs {
     long q_stride, out_stride;
     int B, token_num, Hq, G;
     float score_scale;         // log2(e) / sqrt(D)
-    int nsplit, chunk;         // pieces a tile's rows of the cache are cut into, rows per piece (the last takes the rest)
+    int nsplit;                // pieces a tile's rows of the cache are cut into
     float* part_o;             // [nsplit, token_num * Hq, D]
     float* part_ml;            // [nsplit, token_num * Hq, 2]
 };
 
-// The tile a workgroup works on: tiles are numbered sequence by sequence, the last (longest) tile of the last sequence first.
+// The tile a workgroup works on.  Tiles are numbered longest first, as far as that is cheap to say: the sequences of a block of 64 by
+// their rows, the tiles of a sequence from its end - workgroups start in this order, and the last ones should be short.
+// (eight prompts of 1..2048 tokens in the order they came: 98 us, by length 91.)
 struct Tile {
     int b, first, len, hist;   // sequence, its first packed token, tokens, rows before them
     int m0;                    // first row of the tile: token m / G, head m % G of the group
 };
 
-__device__ __forceinline__ int tiles_of(const PromptArgs& a, int b, int& first, int& len)
-{
-    first = max(a.cu[b], 0);
-    len = min(a.cu[b + 1], a.token_num) - first;
-    if (len <= 0 || a.hist[b] < 0) return 0;
-    return (len * a.G + kRowsPerTile - 1) / kRowsPerTile;
-}
-
 __device__ __forceinline__ bool locate_tile(const PromptArgs& a, int index, Tile& t)
 {
     const int lane = threadIdx.x & (kWave - 1);
-    int total = 0;
-    for (int c = 0; c < a.B; c += kWave) {
-        int first, len;
-        int n = c + lane < a.B ? tiles_of(a, c + lane, first, len) : 0;
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o, kWave);
-        total += n;
-    }
-    if (index >= total) return false;
-    const int want = total - 1 - index;
     int run = 0;
     for (int c = 0; c < a.B; c += kWave) {
-        int first = 0, len = 0;
-        const int n = c + lane < a.B ? tiles_of(a, c + lane, first, len) : 0;
+        int b = c + lane, first = 0, len = 0, hist = 0, n = 0;
+        if (b < a.B) {
+            first = max(a.cu[b], 0);
+            len = min(a.cu[b + 1], a.token_num) - first;
+            hist = a.hist[b];
+            if (len > 0 && hist >= 0) n = (len * a.G + kRowsPerTile - 1) / kRowsPerTile;
+            hist = min(hist, 1 << 30);              // (past every table: all its rows are seen)
+        }
+        const int rows = n > 0 ? hist + len : -1;
+        int rank = 0;                               // sequences with more rows (or as many, and before this one)
+        for (int j = 0; j < min(a.B - c, kWave); ++j) {
+            const int other = __builtin_amdgcn_readlane(rows, j);
+            rank += other > rows || (other == rows && j < lane) ? 1 : 0;
+        }
+        if (b >= a.B) rank = lane;
+        b = __builtin_amdgcn_ds_permute(rank * 4, b);
+        first = __builtin_amdgcn_ds_permute(rank * 4, first);
+        len = __builtin_amdgcn_ds_permute(rank * 4, len);
+        hist = __builtin_amdgcn_ds_permute(rank * 4, hist);
+        n = __builtin_amdgcn_ds_permute(rank * 4, n);
         int inc = n;
 #pragma unroll
         for (int o = 1; o < kWave; o <<= 1) {
             const int up = __shfl_up(inc, o, kWave);
             if (lane >= o) inc += up;
         }
-        const int tot = __shfl(inc, kWave - 1, kWave);
-        if (want < run + tot) {
-            const int f = __builtin_ctzll(__builtin_amdgcn_ballot_w64(run + inc > want));
-            t.b = c + f;
-            t.first = __shfl(first, f, kWave);
-            t.len = __shfl(len, f, kWave);
-            t.m0 = (want - run - __shfl(inc - n, f, kWave)) * kRowsPerTile;
-            t.hist = min(a.hist[t.b], 1 << 30);    // (past every table: all its rows are seen)
+        const int tot = __builtin_amdgcn_readlane(inc, kWave - 1);
+        if (index < run + tot) {
+            const int f = __builtin_ctzll(__builtin_amdgcn_ballot_w64(run + inc > index));
+            t.b = __builtin_amdgcn_readlane(b, f);
+            t.first = __builtin_amdgcn_readlane(first, f);
+            t.len = __builtin_amdgcn_readlane(len, f);
+            t.hist = __builtin_amdgcn_readlane(hist, f);
+            t.m0 = (run + __builtin_amdgcn_readlane(inc, f) - 1 - index) * kRowsPerTile;
             return true;
         }
         run += tot;
@@ -108,13 +110,14 @@ struct PromptShape {
     static constexpr int ND = DP / 32;                      // output tiles
     static constexpr int TILE = BN * ROW;                   // bytes of a staged operand
     static_assert(BN * P % kThreads == 0 && (kWave / P <= kRowGroup), "whole pieces per thread; a wave's pieces lie in one row group");
-    // LDS keeps piece p of row r at p ^ swizzle(r): without it the lanes of a read, which take one piece each of
-    // 16 or more rows, would all hit the same banks
+    // LDS keeps piece p of row r at p ^ swizzle(r): without it the lanes of a read would all hit the same banks.  K: 16 lanes
+    // of a 16-byte read take one piece each of 16 rows.  V, fp16: 32 lanes of a transposed read take 64 bytes each of four rows (a
+    // swizzle that spread only the 16 lanes of one transposition cost two cycles in four); fp32: 32 columns of two rows.
     __device__ static __forceinline__ int swz_k(int r) { return P == 8 ? (r >> 1) & 7 : r & 15; }
     __device__ static __forceinline__ int swz_v(int r)
     {
         if constexpr (!kHalf) return ((r >> 2) & 1) * 8;
-        else return P == 8 ? ((r >> 1) & 3) << 1 : (r & 7) << 1;
+        else return P == 8 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
     }
 };
 
@@ -143,7 +146,8 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
     __shared__ int s_odd;                           // a masked step met a NaN or an infinity in V
 
     Tile t;
-    if (!locate_tile(a, blockIdx.y, t)) return;
+    // (every second piece in the opposite order: workgroups that share a compute unit from the start are a long and a short one)
+    if (!locate_tile(a, blockIdx.z % 2 ? gridDim.y - 1 - blockIdx.y : blockIdx.y, t)) return;
     // the same in every lane: said here, behind the search's loops, so that all that follows from it stays scalar
     t.b = __builtin_amdgcn_readfirstlane(t.b);
     t.first = __builtin_amdgcn_readfirstlane(t.first);
@@ -161,8 +165,9 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
     const int last = __builtin_amdgcn_readfirstlane(min((t.m0 + kRowsPerTile - 1) / a.G, t.len - 1));
     const int rows_end = min(t.hist + last + 1, a.cache.max_pages << a.cache.page_shift);       // rows any row of the tile sees
     const int rows_all = t.hist + __builtin_amdgcn_readfirstlane(t.m0 / a.G) + 1;               // rows every row of it sees
-    const int k_begin = blockIdx.z * a.chunk;
-    const int k_end = blockIdx.z + 1 == (unsigned)a.nsplit ? rows_end : min(k_begin + a.chunk, rows_end);
+    // equal pieces of the tile's own rows, in whole steps
+    const int chunk = a.nsplit == 1 ? rows_end : (__builtin_amdgcn_readfirstlane((rows_end + a.nsplit - 1) / a.nsplit) + 63) / 64 * 64;
+    const int k_begin = blockIdx.z * chunk, k_end = min(k_begin + chunk, rows_end);
     const int limit = min(t.hist + token, k_end - 1);      // the last key the row sees (the table may end before its position)
     const int* table = a.cache.table + (size_t)t.b * a.cache.max_pages;
 
@@ -495,19 +500,49 @@ void paged_prompt_attn_kernel(const PromptArgs a)
     prompt_tile<T, DP>(a);
 }
 
-// Joins the pieces of a split step: one workgroup row per (token, head), four columns per thread.
+// Joins the pieces of a split call: four columns of one (token, head) per thread, four pieces' states in flight at a time.  Whose
+// token it is - one of no sequence has no states and keeps its output - is looked up beside them.
 template <typename T>
 __global__ __launch_bounds__(256)
 void paged_prompt_merge_kernel(const PromptArgs a)
 {
+    constexpr int BATCH = 4;
     const int nq = a.cache.D / 4;                          // (D is a multiple of four)
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
     const long rows = (long)a.token_num * a.Hq;
-    if (i >= rows * nq) return;
-    const long row = i / nq;
-    const int c = (int)(i % nq) * 4;
-    const int token = (int)(row / a.Hq), head = (int)(row % a.Hq);
-    // whose token is it?  (a token of no sequence has no partial states and keeps its output)
+    const int per = 256 / nq;                              // rows of this workgroup
+    const int row = (int)blockIdx.x * per + (int)threadIdx.x / nq, c = (int)threadIdx.x % nq * 4;
+    if ((int)threadIdx.x >= per * nq || row >= rows) return;
+    const int token = row / a.Hq, head = row % a.Hq;
+    float M = -INFINITY, L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < a.nsplit; s0 += BATCH) {
+        float m[BATCH], l[BATCH];
+        f32x4 x[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            const long e = min(s0 + j, a.nsplit - 1) * rows + row;
+            m[j] = a.part_ml[e * 2];
+            l[j] = a.part_ml[e * 2 + 1];
+            x[j] = *reinterpret_cast<const f32x4*>(a.part_o + e * a.cache.D + c);
+        }
+        float bm = M;
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) bm = fmaxf(bm, s0 + j < a.nsplit ? m[j] : -INFINITY);
+        const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - bm) * a.score_scale);
+        L *= keep;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) O[e] *= keep;
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            // (a piece that saw nothing has no weight, whatever its state holds)
+            const bool on = s0 + j < a.nsplit && m[j] != -INFINITY;
+            const float w = on ? __builtin_amdgcn_exp2f((m[j] - bm) * a.score_scale) : 0.f;
+            L = on ? __builtin_fmaf(l[j], w, L) : L;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[e] = on ? __builtin_fmaf(x[j][e], w, O[e]) : O[e];
+        }
+        M = bm;
+    }
     int lo = 0, hi = a.B;                                  // the first b with cu[b + 1] > token
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
@@ -515,19 +550,6 @@ void paged_prompt_merge_kernel(const PromptArgs a)
         else hi = mid;
     }
     if (lo >= a.B || token < a.cu[lo] || a.hist[lo] < 0) return;
-    float M = -INFINITY;
-    for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, a.part_ml[(s * rows + row) * 2]);
-    float L = 0.f;
-    f32x4 O = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float m = a.part_ml[(s * rows + row) * 2];
-        if (m == -INFINITY) continue;                      // a piece that saw nothing
-        const float w = __builtin_amdgcn_exp2f((m - M) * a.score_scale);
-        L = __builtin_fmaf(a.part_ml[(s * rows + row) * 2 + 1], w, L);
-        const f32x4 p = *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * a.cache.D + c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) O[e] = __builtin_fmaf(p[e], w, O[e]);
-    }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     T* out = static_cast<T*>(a.out) + (size_t)token * a.out_stride + (size_t)head * a.cache.D + c;
 #pragma unroll
@@ -543,8 +565,8 @@ int launch_prompt(const PromptArgs& a, int tiles, hipStream_t st)
     else hipLaunchKernelGGL((paged_prompt_attn_kernel<T, 256>), grid, dim3(kThreads), 0, st, a);
     int rc = launch_status();
     if (rc || a.nsplit == 1) return rc;
-    const long n = (long)a.token_num * a.Hq * (a.cache.D / 4);
-    hipLaunchKernelGGL((paged_prompt_merge_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    const int rows = a.token_num * a.Hq, per = 256 / (a.cache.D / 4);
+    hipLaunchKernelGGL((paged_prompt_merge_kernel<T>), dim3((rows + per - 1) / per), dim3(256), 0, st, a);
     return launch_status();
 }
 
@@ -555,13 +577,19 @@ long tiles_bound(int B, int token_num, int G)
     return rows / kRowsPerTile + (token_num < B ? token_num : B);
 }
 
-// Pieces the rows of the cache are cut into: none while the tiles alone fill the chip (two workgroups per compute unit),
-// else as many as fill it, of 512 rows or more each.
-int split_of(long tiles, int Hkv, int max_rows)
+// Pieces the rows of the cache are cut into: none while the tiles alone keep the chip busy, else as many as give two workgroups
+// per compute unit, of 512 rows or more each - a second launch and the states' way through memory have to be worth it.
+// 461 tokens behind 15000..20000 rows (128 tiles, fp16): 3 / 4 / 5 / 7 pieces 197 / 181 / 194 / 190 us.
+// fp32: a tile's steps take six times as long, so the longest tile of a call ends long after the others unless it is cut:
+// four workgroups per compute unit, pieces of 128 rows (2058 tokens, 258 tiles of up to 1324 rows: uncut 89 us, two pieces 94,
+// four 76, eight 82).
+int split_of(int dtype, long tiles, int Hkv, int max_rows)
 {
-    const long wgs = tiles * Hkv;
-    long n = 512 / (wgs < 1 ? 1 : wgs);
-    const long most = max_rows / 512;
+    const bool half = dtype == ONELLM_FP16;
+    const long wgs = tiles * Hkv < 1 ? 1 : tiles * Hkv, target = half ? 512 : 1024;
+    if (half && wgs > 256) return 1;
+    long n = (target + wgs / 2) / wgs;
+    const long most = max_rows / (half ? 512 : 128);
     if (n > most) n = most;
     return n < 1 ? 1 : (int)n;
 }
@@ -573,7 +601,7 @@ extern "C" size_t onellm_paged_prompt_attn_workspace_bytes(int B, int token_num,
 {
     using namespace onellm;
     if (B <= 0 || token_num <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || max_rows <= 0) return 256;
-    const int n = split_of(tiles_bound(B, token_num, Hq / Hkv), Hkv, max_rows);
+    const int n = split_of(ONELLM_FP32, tiles_bound(B, token_num, Hq / Hkv), Hkv, max_rows);     // (fp16: never more)
     if (n == 1) return 256;
     return (((size_t)n * token_num * Hq * (D + 2) * sizeof(float)) + 255) / 256 * 256;
 }
@@ -612,8 +640,7 @@ extern "C" int onellm_paged_prompt_attn(int dtype, const void* q, long q_stride,
     a.Hq = Hq;
     a.G = G;
     a.score_scale = 1.44269504088896340736f / sqrtf((float)D);
-    a.nsplit = split_of(tiles, Hkv, max_rows);
-    a.chunk = ((max_rows + a.nsplit - 1) / a.nsplit + 63) / 64 * 64;
+    a.nsplit = split_of(dtype, tiles, Hkv, max_rows);
     a.part_o = nullptr;
     a.part_ml = nullptr;
     if (a.nsplit > 1) {

@@ -123,7 +123,7 @@ def test_no_tokens_is_no_work(capi):
 
 def test_workspace_sizes(capi):
     size = capi.paged_prompt_attn_workspace_bytes
-    assert size(1, 8192, 32, 8, 128, 8192) == 256                     # enough tiles: nothing is cut
+    assert size(1, 8192, 32, 8, 128, 8192) == 256                     # enough tiles: nothing is cut in either type
     n = size(1, 8, 32, 8, 128, 32768)
     assert n % 256 == 0 and n >= 2 * 8 * 32 * 130 * 4
     assert size(0, 8, 32, 8, 128, 32768) == 256 and size(1, 8, 32, 7, 128, 100) == 256
