@@ -95,6 +95,9 @@ __device__ __forceinline__ f32x4 join_waves(const float* st_ml, const float* acc
     return O;
 }
 
+// two neighbouring columns of a row
+template <typename T> struct alignas(2 * sizeof(T)) Pair { T a, b; };
+
 template <typename T>
 __device__ __forceinline__ void store_quad(T* out, f32x4 v)
 {
@@ -178,89 +181,70 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
                                                           __builtin_amdgcn_raw_buffer_load_b128(w, voff[cg], e * D * (int)sizeof(T), kStream));
         }
     };
+    // ---- the new token: q of the tile's heads, and in the last piece its k and v row, a pair of columns per thread at a
+    // time, two pairs' loads together.  The first ones set out before the rows' first loads: loads return in order, and the set-up
+    // then runs while the rows are on their way (behind them it waited for 64 KiB per compute unit).
+    const int QKVH = a.Hq + 2 * a.Hkv;
+    const T* qkv = static_cast<const T*>(p.qkv) + (size_t)u.b * QKVH * D;
+    const T* bias = static_cast<const T*>(p.bias);
+    const int pos = u.t - 1, half_d = D / 2;
+    const int rows_new = ng + (u.is_last ? 2 : 0);            // heads of q, then k, then v
+    Pair<T> nx[2], ny[2];
+    int ng_[2], npair[2];
+    auto request_new = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = min(i0 + j * kThr, rows_new * half_d - 1);
+            ng_[j] = i / half_d;
+            npair[j] = i - ng_[j] * half_d;
+            const int head = ng_[j] < ng ? u.kvh * a.G + u.g0 + ng_[j] : a.Hq + u.kvh + (ng_[j] - ng) * a.Hkv;
+            nx[j] = *reinterpret_cast<const Pair<T>*>(qkv + head * D + 2 * npair[j]);
+            ny[j] = bias ? *reinterpret_cast<const Pair<T>*>(bias + head * D + 2 * npair[j]) : Pair<T>{};
+        }
+    };
+    request_new(tid);
+    asm volatile("" ::: "memory");                            // (the requests stay in front of the rows')
+
     int rb = u.r0 + wave * RW;
     Pages now = fetch_pages(rb);
     issue_k(now, rb);
     issue_v(now, rb);
     Pages next = fetch_pages(rb + S::RPI);
 
-    // ---- the new token: q of the tile's heads, and in the last piece its k and v rows
-    const int QKVH = a.Hq + 2 * a.Hkv;
-    const T* qkv = static_cast<const T*>(p.qkv) + (size_t)u.b * QKVH * D;
-    const T* bias = static_cast<const T*>(p.bias);
-    const int pos = u.t - 1;
-    for (int i = tid; i < kHeads * (DP / 2); i += kThr) {
-        const int g = i / (DP / 2), pr = i % (DP / 2);
-        float x0 = 0.f, x1 = 0.f;
-        if (g < ng && 2 * pr < D) {
-            const int o = (u.kvh * a.G + u.g0 + g) * D + 2 * pr;
-            x0 = to_f32(qkv[o]);
-            x1 = to_f32(qkv[o + 1]);
-            if (bias) {
-                x0 += to_f32(bias[o]);
-                x1 += to_f32(bias[o + 1]);
+    const int new_page = u.is_last ? page_of(p.cache, table, pos) : -1;
+    const bool keep = u.g0 == 0 && new_page >= 0;
+    const size_t new_at = keep ? paged_offset(p.cache, new_page, u.kvh, pos) : 0;
+    for (int i0 = tid; i0 < rows_new * half_d; i0 += 2 * kThr) {
+        if (i0 != tid) request_new(i0);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if (i0 + j * kThr >= rows_new * half_d) continue;
+            const int g = ng_[j], pr = npair[j];
+            float x0 = to_f32(nx[j].a) + (bias ? to_f32(ny[j].a) : 0.f), x1 = to_f32(nx[j].b) + (bias ? to_f32(ny[j].b) : 0.f);
+            if (g <= ng && 2 * pr < a.rotary_dim) {
+                float sn, cs;
+                rope_sincos(pos, rt.f[pr], sn, cs);
+                const float r0 = __builtin_fmaf(x0, cs, -(x1 * sn));
+                x1 = __builtin_fmaf(x1, cs, x0 * sn);
+                x0 = r0;
             }
-            if (2 * pr < a.rotary_dim) {
-                float s, c;
-                rope_sincos(pos, rt.f[pr], s, c);
-                const float y0 = __builtin_fmaf(x0, c, -(x1 * s));
-                x1 = __builtin_fmaf(x1, c, x0 * s);
-                x0 = y0;
+            if (g < ng) {
+                sq[g * DP + 2 * pr] = x0 * a.qscale;
+                sq[g * DP + 2 * pr + 1] = x1 * a.qscale;
+            } else {
+                const Pair<T> v{from_f32<T>(x0), from_f32<T>(x1)};
+                float* d = g == ng ? sk : sv;                 // the row as the cache holds it
+                d[2 * pr] = to_f32(v.a);
+                d[2 * pr + 1] = to_f32(v.b);
+                if (keep) *reinterpret_cast<Pair<T>*>(static_cast<T*>(g == ng ? p.k_pages : p.v_pages) + new_at + 2 * pr) = v;
             }
-        }
-        sq[g * DP + 2 * pr] = x0 * a.qscale;
-        sq[g * DP + 2 * pr + 1] = x1 * a.qscale;
-    }
-    if (u.is_last) {
-        const int page = page_of(p.cache, table, pos);
-        const bool keep = u.g0 == 0 && page >= 0;
-        const size_t at = keep ? paged_offset(p.cache, page, u.kvh, pos) : 0;
-        for (int pr = tid; pr < DP / 2; pr += kThr) {
-            float x0 = 0.f, x1 = 0.f, y0 = 0.f, y1 = 0.f;
-            if (2 * pr < D) {
-                const int ok = (a.Hq + u.kvh) * D + 2 * pr, ov = ok + a.Hkv * D;
-                x0 = to_f32(qkv[ok]);
-                x1 = to_f32(qkv[ok + 1]);
-                y0 = to_f32(qkv[ov]);
-                y1 = to_f32(qkv[ov + 1]);
-                if (bias) {
-                    x0 += to_f32(bias[ok]);
-                    x1 += to_f32(bias[ok + 1]);
-                    y0 += to_f32(bias[ov]);
-                    y1 += to_f32(bias[ov + 1]);
-                }
-                if (2 * pr < a.rotary_dim) {
-                    float s, c;
-                    rope_sincos(pos, rt.f[pr], s, c);
-                    const float z0 = __builtin_fmaf(x0, c, -(x1 * s));
-                    x1 = __builtin_fmaf(x1, c, x0 * s);
-                    x0 = z0;
-                }
-                const T k0 = from_f32<T>(x0), k1 = from_f32<T>(x1), v0 = from_f32<T>(y0), v1 = from_f32<T>(y1);
-                if (keep) {
-                    T* kd = static_cast<T*>(p.k_pages) + at + 2 * pr;
-                    T* vd = static_cast<T*>(p.v_pages) + at + 2 * pr;
-                    kd[0] = k0;
-                    kd[1] = k1;
-                    vd[0] = v0;
-                    vd[1] = v1;
-                }
-                x0 = to_f32(k0);                              // the row as the cache holds it
-                x1 = to_f32(k1);
-                y0 = to_f32(v0);
-                y1 = to_f32(v1);
-            }
-            sk[2 * pr] = x0;
-            sk[2 * pr + 1] = x1;
-            sv[2 * pr] = y0;
-            sv[2 * pr + 1] = y1;
         }
     }
     __syncthreads();
     if (u.is_last) {
-        for (int g = wave; g < kHeads; g += kWaves) {
+        for (int g = wave; g < ng; g += kWaves) {
             float part = 0.f;
-            for (int d = lane; d < DP; d += kWave) part = __builtin_fmaf(sq[g * DP + d], sk[d], part);
+            for (int d = lane; d < D; d += kWave) part = __builtin_fmaf(sq[g * DP + d], sk[d], part);
             part = wave_sum(part);
             if (lane == 0) snew[g] = part;
         }
@@ -273,7 +257,7 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
     for (int j = 0; j < NKJ; ++j)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            const float v = sq[slot * DP + (grp + 4 * j) * VEC + e];
+            const float v = slot < ng && (grp + 4 * j) * VEC < D ? sq[slot * DP + (grp + 4 * j) * VEC + e] : 0.f;
             if constexpr (S::kHalf) {
                 qhi[j][e] = (_Float16)v;
                 qlo[j][e] = (_Float16)(v - (float)qhi[j][e]);
@@ -448,46 +432,69 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
     if (*arrived != P - 1) return;
     if (tid == 0) __hip_atomic_store(p.counters + i0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);    // zero for the next call
 
-    // weights of the pieces, a head per wave: 2^(m - M) / L
+    // The first batch of sums sets out beside the statistics; their weights - 2^(m - M) / L, a head per wave - are worked out
+    // meanwhile.  A thread takes a quad of columns and, where there are fewer quads than threads, every `slices`-th batch of pieces.
+    constexpr int BATCH = 4;
+    const int quads = ng * nq, slices = max(1, kThr / quads);
+    const int quad = tid % quads, slice = tid / quads;
     float* wgt = scratch;                                     // [P][ng]
-    for (int g = wave; g < ng; g += kWaves) {
-        float M = -INFINITY;
-        for (int s = lane; s < P; s += kWave) {
-            const auto ml = __builtin_amdgcn_raw_buffer_load_b64(wm, entry(i0 + s, g) * 8u, 0, kDevice);
-            M = fmaxf(M, __uint_as_float(ml[0]));
-        }
-#pragma unroll
-        for (int x = 32; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, kWave));
-        float L = 0.f;
-        for (int s = lane; s < P; s += kWave) {
-            const auto ml = __builtin_amdgcn_raw_buffer_load_b64(wm, entry(i0 + s, g) * 8u, 0, kDevice);
-            L += __uint_as_float(ml[1]) * __builtin_amdgcn_exp2f(__uint_as_float(ml[0]) - M);
-        }
-        L = wave_sum(L);
-        for (int s = lane; s < P; s += kWave) {
-            const auto ml = __builtin_amdgcn_raw_buffer_load_b64(wm, entry(i0 + s, g) * 8u, 0, kDevice);
-            wgt[s * ng + g] = __builtin_amdgcn_exp2f(__uint_as_float(ml[0]) - M) / L;
-        }
-    }
-    __syncthreads();
-    for (int i = tid; i < ng * nq; i += kThr) {
-        const int g = i / nq, c = (i % nq) * 4;
-        f32x4 O = {0.f, 0.f, 0.f, 0.f};
-        constexpr int BATCH = 8;
-        for (int s0 = 0; s0 < P; s0 += BATCH) {
-            u32x4 x[BATCH];
+    f32x4* part = reinterpret_cast<f32x4*>(lds);              // [slices][quads] (q and the new rows are no longer needed)
+    const int rounds = (quads + kThr - 1) / kThr;
+    for (int round = 0; round < rounds; ++round) {
+        const int i = slices > 1 ? quad : tid + round * kThr;
+        const bool on = slices > 1 ? slice < slices : i < quads;
+        const int g = on ? i / nq : 0, c = on ? (i - g * nq) * 4 : 0;
+        const int first = slices > 1 ? slice : 0;
+        u32x4 x[BATCH];
+        auto fetch = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < BATCH; ++j)
                 x[j] = __builtin_amdgcn_raw_buffer_load_b128(wo, (entry(i0 + min(s0 + j, P - 1), g) * D + c) * 4u, 0, kDevice);
+        };
+        fetch(first * BATCH);
+        if (round == 0) {
+            for (int h = wave; h < ng; h += kWaves) {
+                float M = -INFINITY, L = 0.f;
+                for (int s = lane; s < P; s += kWave) {
+                    const auto ml = __builtin_amdgcn_raw_buffer_load_b64(wm, entry(i0 + s, h) * 8u, 0, kDevice);
+                    const float pm = __uint_as_float(ml[0]), pl = __uint_as_float(ml[1]);
+                    wgt[s * ng + h] = pm;
+                    const float top = fmaxf(M, pm);           // (a piece that saw nothing: -inf, and no sum)
+                    const float base = top == -INFINITY ? 0.f : top;
+                    L = L * __builtin_amdgcn_exp2f(M - base) + pl * __builtin_amdgcn_exp2f(pm - base);
+                    M = top;
+                }
+                float top = M;
+#pragma unroll
+                for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, kWave));
+                L = wave_sum(L * __builtin_amdgcn_exp2f(M - top));           // (the new token's piece has a finite maximum)
+                for (int s = lane; s < P; s += kWave) wgt[s * ng + h] = __builtin_amdgcn_exp2f(wgt[s * ng + h] - top) / L;
+            }
+            __syncthreads();
+        }
+        f32x4 O = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = first * BATCH; s0 < P; s0 += slices * BATCH) {
+            if (s0 != first * BATCH) fetch(s0);
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
-                const float f = s0 + j < P ? wgt[min(s0 + j, P - 1) * ng + g] : 0.f;
+                const float f = wgt[min(s0 + j, P - 1) * ng + g];
                 const f32x4 y = __builtin_bit_cast(f32x4, x[j]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) O[e] = s0 + j < P ? __builtin_fmaf(y[e], f, O[e]) : O[e];
             }
         }
-        store_quad<T>(out + (size_t)g * D + c, O);
+        if (slices > 1) {
+            if (on) part[slice * quads + quad] = O;
+            __syncthreads();
+            if (slice == 0) {
+                for (int x = 1; x < min(slices, (P + BATCH - 1) / BATCH); ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) O[e] += part[x * quads + quad][e];
+                store_quad<T>(out + (size_t)g * D + c, O);
+            }
+        } else if (on) {
+            store_quad<T>(out + (size_t)g * D + c, O);
+        }
     }
 }
 
@@ -571,8 +578,17 @@ extern "C" int onellm_paged_decode_attn(int dtype, const void* qkv, const void* 
     a.rotary_dim = rotary_dim;
     a.qscale = 1.44269504088896340736f / sqrtf((float)D);
     a.item_rows = 64;
-    a.bal_nwg = kBalancedWorkgroups;
-    a.unit_cost = 3;
+    // One share per compute unit, two where there are many short units (a second workgroup then covers the first one's set-up and
+    // finish; with long units the two end far apart).  16 sequences x 32 kv heads of 128, fp16, one / two shares: 512 rows
+    // 29.0 / 24.6 us, 1024 rows 48.4 / 44.7, 4096 rows 163.4 / 167.6; 96 x 8 heads of 100..1000 rows 54.6 / 50.9; 32 x 8 of
+    // 1024..8192 rows 100.1 / 101.4; 8 x 8 of 256..2048 rows 16.2 / 18.9; 32 x 8 heads of 64, 512..4096 rows 39.5 / 38.3.
+    // A change of unit costs a workgroup about 1.5 KiB x 64 of each cache's bytes, half that where another workgroup fills in.
+    const long long row_bytes = (long long)D * (dtype == ONELLM_FP16 ? 2 : 4);
+    const bool two = units >= kBalancedWorkgroups / 2 && longest * row_bytes <= 512 << 10;
+    a.bal_nwg = two ? kBalancedWorkgroups : kBalancedWorkgroups / 2;
+    a.unit_cost = (int)((two ? 768 : 1536) / row_bytes);
+    if (a.unit_cost < 1) a.unit_cost = 1;
+    if (a.unit_cost > 12) a.unit_cost = 12;
     // item numbers times workgroups have to stay below 2^31 (attn_schedule.hpp)
     while (units * ((longest - 1 + a.item_rows - 1) / a.item_rows + 1 + a.unit_cost) * a.bal_nwg > (long long)kBalancedMaxItemsTimesWorkgroups) {
         if (a.item_rows >= 1 << 20) return ONELLM_EUNSUPPORTED;
