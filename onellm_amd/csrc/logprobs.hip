@@ -9,9 +9,8 @@
 // half a slot for the maximum that is 6.5 slots, 22 us for 4096 x 32000 logits on all SIMDs against 37 us to read them in fp16.
 //
 // The K best: a wave keeps candidates in LDS as 64-bit keys (value, then lower token first).  The K-th largest of its
-// lanes' maxima, found bit by bit with ballots, is a floor below which nothing can be among the K best; a 16-byte piece whose maximum
-// reaches the floor is looked through, its candidates appended, and the list cut back to the K best, which
-// raises the floor.  Ties and sorted rows only make the list be cut back more often.
+// lanes' maxima, found bit by bit with ballots, is a floor below which nothing can be among the K best; the lanes that reach
+// it are looked through, their candidates appended, and the list cut back to the K best, which raises the floor.  Ties and sorted rows only make the list be cut back more often.
 //
 // Few rows are cut into parts, a workgroup each, and joined by a second launch.
 #include "common.hpp"
@@ -27,6 +26,7 @@ constexpr int kThr = 256, kWaves = kThr / kWave;
 constexpr int kPieces = 8;                     // 16-byte pieces per thread and step
 constexpr int kMaxK = 32;
 constexpr int kList = 256;                     // candidates a wave keeps
+constexpr int kStage = 16;                     // lanes whose logits are looked through together
 constexpr int kMaxParts = 16;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr unsigned kNegInfKey = 0x007FFFFFu;   // the key word of -inf
@@ -162,6 +162,7 @@ void token_logprobs_kernel(const LogprobArgs a)
 {
     constexpr int VEC = Elt<T>::kVec;
     __shared__ Key lists[TOP ? kWaves : 1][TOP ? kList : 1];
+    __shared__ __align__(16) char stage[TOP ? kWaves : 1][TOP ? kStage : 1][kPieces * 16 + 16];
     __shared__ int counts[kWaves];
     __shared__ Stats stats[kWaves];
     const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
@@ -204,7 +205,7 @@ void token_logprobs_kernel(const LogprobArgs a)
                 }
             }
         }
-        float pm[kPieces], lm = -INFINITY;    // maxima of the pieces, of the lane
+        float lm = -INFINITY;                 // the lane's maximum
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             if constexpr (sizeof(T) == 2) {
@@ -212,11 +213,10 @@ void token_logprobs_kernel(const LogprobArgs a)
                 h = __builtin_elementwise_max(h, __builtin_shufflevector(v[i].raw, v[i].raw, 2, 3));
                 h = __builtin_elementwise_max(h, __builtin_shufflevector(v[i].raw, v[i].raw, 4, 5));
                 h = __builtin_elementwise_max(h, __builtin_shufflevector(v[i].raw, v[i].raw, 6, 7));
-                pm[i] = fmaxf((float)h[0], (float)h[1]);
+                lm = fmaxf(lm, fmaxf((float)h[0], (float)h[1]));
             } else {
-                pm[i] = fmaxf(fmaxf(v[i].get(0), v[i].get(1)), fmaxf(v[i].get(2), v[i].get(3)));
+                lm = fmaxf(lm, fmaxf(fmaxf(v[i].get(0), v[i].get(1)), fmaxf(v[i].get(2), v[i].get(3))));
             }
-            lm = fmaxf(lm, pm[i]);
         }
         const float ref = fmaxf(st.ref, reference_of<T>(lm));
         const float old = st.ref == ref ? 0.f : fmaxf(exponent_between<T>(st.ref, ref), -1e4f);
@@ -244,30 +244,45 @@ void token_logprobs_kernel(const LogprobArgs a)
                 if (t > kNegInfKey) floor_v = value_of(t);
                 have_floor = true;
             }
+            // the lanes whose maximum reaches the floor put their logits into LDS, kStage lanes at a time, where the whole wave
+            // looks through one lane's (fp32: two lanes') at once
             bool cut = false;
+            unsigned long long who = __builtin_amdgcn_ballot_w64(lm >= floor_v && lm > -INFINITY);
+            while (who) {
+                const int rank = __builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0u));
+                const bool mine = (who >> lane & 1) && rank < kStage;
+                const unsigned long long now = __builtin_amdgcn_ballot_w64(mine);
+                if (mine) {
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                if (__builtin_amdgcn_ballot_w64(pm[i] >= floor_v && pm[i] > -INFINITY) == 0) continue;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float q = v[i].get(e);
-                    const int id = c0 + (i * kThr + tid) * VEC + e;
-                    const bool is = q > -INFINITY && (q > floor_v || (q == floor_v && id <= floor_id));
-                    const unsigned long long who = __builtin_amdgcn_ballot_w64(is);
-                    if (who == 0) continue;
-                    const int n = __builtin_popcountll(who);
-                    if (count + n > kList) {
+                    for (int i = 0; i < kPieces; ++i) *reinterpret_cast<decltype(v[i].raw)*>(stage[wave][rank] + i * 16) = v[i].raw;
+                    *reinterpret_cast<int*>(stage[wave][rank] + kPieces * 16) = lane;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                const int n = __builtin_popcountll(now);
+                constexpr int EL = kPieces * VEC, AT_ONCE = kWave / EL;        // logits of a lane; lanes looked through at once
+                for (int c = 0; c < n; c += AT_ONCE) {
+                    const int from = c + lane / EL, j = lane % EL;
+                    const char* s = stage[wave][min(from, n - 1)];
+                    const float q = to_f32(reinterpret_cast<const T*>(s)[j]);
+                    const int id = c0 + ((j / VEC) * kThr + wave * kWave + *reinterpret_cast<const int*>(s + kPieces * 16)) * VEC + j % VEC;
+                    const bool is = from < n && q > -INFINITY && (q > floor_v || (q == floor_v && id <= floor_id));
+                    const unsigned long long hits = __builtin_amdgcn_ballot_w64(is);
+                    if (hits == 0) continue;
+                    if (count + __builtin_popcountll(hits) > kList) {
                         count = cut_list<kList / kWave>(list, count, a.K);
                         if (count == a.K) {
                             floor_v = value_of((unsigned)(list[a.K - 1] >> 32));
                             floor_id = id_of(list[a.K - 1]);
                         }
                     }
-                    const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0u));
+                    const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(hits >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hits, 0u));
                     if (is) list[count + before] = make_key(q, id);
-                    count += n;
+                    count += __builtin_popcountll(hits);
                     cut = true;
                 }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                who &= ~now;
+                who &= __builtin_amdgcn_ballot_w64(lm >= floor_v);             // (a cut may have raised it)
             }
             if (cut) {
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
