@@ -8,8 +8,8 @@
 // Per logit that is a multiply-add, an exponential (two issue slots), an add and for the entropy a clamp and a multiply-add; with
 // half a slot for the maximum that is 6.5 slots, 22 us for 4096 x 32000 logits on all SIMDs against 37 us to read them in fp16.
 //
-// The K best: a wave keeps candidates in LDS as 64-bit keys (value, then lower token first).  The K-th largest of its
-// lanes' maxima, found bit by bit with ballots, is a floor below which nothing can be among the K best; the lanes that reach
+// The K best: a wave keeps candidates in LDS as 64-bit keys (value, then lower token first).  The K-th largest of the first step's
+// 256 lane maxima, found bit by bit with ballots, is a floor below which nothing can be among the K best; the lanes that reach
 // it are looked through, their candidates appended, and the list cut back to the K best, which raises the floor.  Ties and sorted rows only make the list be cut back more often.
 //
 // Few rows are cut into parts, a workgroup each, and joined by a second launch.
@@ -104,18 +104,62 @@ __device__ __forceinline__ Stats join_wave(Stats a)
     return a;
 }
 
-// Cuts a list of n <= 64 * PER keys, all different, to its k best, in order.  Called by one whole wave.
+// Cuts a list of n <= 64 * PER keys, all different, to its k best, in order.  Called by one whole wave.  Up to 64 keys are ranked
+// out of registers, every key read out of its lane and compared in all of them.  Of a longer list first the keys below the k-th largest
+// value are dropped, that value found bit by bit; if ties leave more than 64, the list is ranked against itself in LDS.
+__device__ __forceinline__ int rank_list(Key* list, int n, int k)
+{
+    const int lane = threadIdx.x & (kWave - 1);
+    const Key own = lane < n ? list[lane] : 0;
+    int rank = 0;
+    for (int i0 = 0; i0 < n; i0 += 8) {                       // (keys behind the list are 0, above nothing)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const Key x = (Key)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(own >> 32), i0 + i) << 32
+                          | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)own, i0 + i);
+            rank += x > own ? 1 : 0;
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (lane < n && rank < k) list[rank] = own;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    return min(n, k);
+}
+
 template <int PER>
 __device__ __forceinline__ int cut_list(Key* list, int n, int k)
 {
+    if (n <= kWave) return rank_list(list, n, k);
     const int lane = threadIdx.x & (kWave - 1);
     Key own[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) own[j] = lane + j * kWave < n ? list[lane + j * kWave] : 0;
+    unsigned t = 0;                                           // the k-th largest value (k <= 32 < n)
+    for (unsigned bit = 0x80000000u; bit; bit >>= 1) {
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64((unsigned)(own[j] >> 32) >= (t | bit)));
+        if (c >= k) t |= bit;
+    }
+    int left = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) left += __builtin_popcountll(__builtin_amdgcn_ballot_w64((unsigned)(own[j] >> 32) >= t));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (left <= kWave) {
+        int at = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const bool on = (unsigned)(own[j] >> 32) >= t;
+            const unsigned long long who = __builtin_amdgcn_ballot_w64(on);
+            if (on) list[at + __builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0u))] = own[j];
+            at += __builtin_popcountll(who);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        return rank_list(list, left, k);
+    }
     int rank[PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        own[j] = lane + j * kWave < n ? list[lane + j * kWave] : 0;
-        rank[j] = 0;
-    }
+    for (int j = 0; j < PER; ++j) rank[j] = 0;
     for (int i = 0; i < n; ++i) {
         const Key x = list[i];
 #pragma unroll
@@ -163,9 +207,10 @@ void token_logprobs_kernel(const LogprobArgs a)
     constexpr int VEC = Elt<T>::kVec;
     __shared__ Key lists[TOP ? kWaves : 1][TOP ? kList : 1];
     __shared__ __align__(16) char stage[TOP ? kWaves : 1][TOP ? kStage : 1][kPieces * 16 + 16];
+    __shared__ float lane_max[TOP ? kWaves : 1][TOP ? kWave : 1];
     __shared__ int counts[kWaves];
     __shared__ Stats stats[kWaves];
-    const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const int row = blockIdx.x, part = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const T* x = static_cast<const T*>(a.logits) + (size_t)row * a.ld;
     // 16-byte pieces are taken from the aligned address at or before the row's first logit; a piece that is not wholly
@@ -236,11 +281,19 @@ void token_logprobs_kernel(const LogprobArgs a)
             }
         if constexpr (TOP) {
             if (!have_floor) {
-                // the K-th largest lane maximum, its 18 leading bits
-                const unsigned o = order_of(lm);
+                // the K-th largest of the workgroup's lane maxima, its 18 leading bits (every wave works it out for itself)
+                lane_max[wave][lane] = lm;
+                __syncthreads();
+                unsigned o[kWaves];
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) o[w] = order_of(lane_max[w][lane]);
                 unsigned t = 0;
-                for (unsigned bit = 0x80000000u; bit >= 0x4000u; bit >>= 1)
-                    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(o >= (t | bit))) >= a.K) t |= bit;
+                for (unsigned bit = 0x80000000u; bit >= 0x4000u; bit >>= 1) {
+                    int n = 0;
+#pragma unroll
+                    for (int w = 0; w < kWaves; ++w) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(o[w] >= (t | bit)));
+                    if (n >= a.K) t |= bit;
+                }
                 if (t > kNegInfKey) floor_v = value_of(t);
                 have_floor = true;
             }
@@ -260,33 +313,41 @@ void token_logprobs_kernel(const LogprobArgs a)
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 const int n = __builtin_popcountll(now);
                 constexpr int EL = kPieces * VEC, AT_ONCE = kWave / EL;        // logits of a lane; lanes looked through at once
-                for (int c = 0; c < n; c += AT_ONCE) {
-                    const int from = c + lane / EL, j = lane % EL;
-                    const char* s = stage[wave][min(from, n - 1)];
-                    const float q = to_f32(reinterpret_cast<const T*>(s)[j]);
-                    const int id = c0 + ((j / VEC) * kThr + wave * kWave + *reinterpret_cast<const int*>(s + kPieces * 16)) * VEC + j % VEC;
-                    const bool is = from < n && q > -INFINITY && (q > floor_v || (q == floor_v && id <= floor_id));
-                    const unsigned long long hits = __builtin_amdgcn_ballot_w64(is);
-                    if (hits == 0) continue;
-                    if (count + __builtin_popcountll(hits) > kList) {
-                        count = cut_list<kList / kWave>(list, count, a.K);
-                        if (count == a.K) {
-                            floor_v = value_of((unsigned)(list[a.K - 1] >> 32));
-                            floor_id = id_of(list[a.K - 1]);
-                        }
+                for (int at = 0; at < n; at += 4 * AT_ONCE) {               // (four reads in flight)
+                    float q[4];
+                    int id[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int from = at + u * AT_ONCE + lane / EL, j = lane % EL;
+                        const char* s = stage[wave][min(from, n - 1)];
+                        q[u] = from < n ? to_f32(reinterpret_cast<const T*>(s)[j]) : -INFINITY;
+                        id[u] = c0 + ((j / VEC) * kThr + wave * kWave + *reinterpret_cast<const int*>(s + kPieces * 16)) * VEC + j % VEC;
                     }
-                    const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(hits >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hits, 0u));
-                    if (is) list[count + before] = make_key(q, id);
-                    count += __builtin_popcountll(hits);
-                    cut = true;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const bool is = q[u] > -INFINITY && (q[u] > floor_v || (q[u] == floor_v && id[u] <= floor_id));
+                        const unsigned long long hits = __builtin_amdgcn_ballot_w64(is);
+                        if (hits == 0) continue;
+                        if (count + __builtin_popcountll(hits) > kList) {
+                            count = cut_list<kList / kWave>(list, count, a.K);
+                            if (count == a.K) {
+                                floor_v = value_of((unsigned)(list[a.K - 1] >> 32));
+                                floor_id = id_of(list[a.K - 1]);
+                            }
+                        }
+                        const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(hits >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hits, 0u));
+                        if (is) list[count + before] = make_key(q[u], id[u]);
+                        count += __builtin_popcountll(hits);
+                        cut = true;
+                    }
                 }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 who &= ~now;
                 who &= __builtin_amdgcn_ballot_w64(lm >= floor_v);             // (a cut may have raised it)
             }
-            if (cut) {
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                count = count <= kWave ? cut_list<1>(list, count, a.K) : cut_list<kList / kWave>(list, count, a.K);
+            // (a list of up to 64 is cut once, behind the last step: a floor that is a little low costs less than the cut)
+            if (cut && count > kWave) {
+                count = cut_list<kList / kWave>(list, count, a.K);
                 if (count == a.K) {
                     floor_v = value_of((unsigned)(list[a.K - 1] >> 32));
                     floor_id = id_of(list[a.K - 1]);
@@ -295,6 +356,7 @@ void token_logprobs_kernel(const LogprobArgs a)
         }
     }
 
+    if constexpr (TOP) count = rank_list(list, count, a.K);       // (64 keys at most)
     st = join_wave<T>(st);
     if (lane == 0) {
         stats[wave] = st;
@@ -350,15 +412,16 @@ void token_logprobs_join_kernel(const LogprobArgs a)
     }
     st = join_wave<T>(st);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (a.K) n = n <= kWave ? cut_list<1>(list, n, a.K) : cut_list<kMaxParts * kMaxK / kWave>(list, n, a.K);
+    if (a.K) n = cut_list<kMaxParts * kMaxK / kWave>(list, n, a.K);
     write_row<T>(a, row, st, list, n, lane);
 }
 
-// Parts per row: one while the rows alone give every compute unit two workgroups, else enough for that, of two steps or more each.
+// Parts per row: one while the rows alone give every compute unit two workgroups, else enough for that, of a step or more each
+// (16 x 32000 fp16, K = 8: two parts of two steps 16.1 us, four of one 12.1; 64 x 128000: 20.4, 15.3).
 int parts_of(int N, int V, int step)
 {
     int n = N >= 512 ? 1 : (511 + N) / N;
-    const int most = (V + 2 * step - 1) / (2 * step);
+    const int most = (V + step - 1) / step;
     if (n > most) n = most;
     return n < 1 ? 1 : (n > kMaxParts ? kMaxParts : n);
 }
@@ -366,7 +429,7 @@ int parts_of(int N, int V, int step)
 template <typename T>
 int launch_logprobs(const LogprobArgs& a, hipStream_t st)
 {
-    const dim3 grid((unsigned)a.N * (unsigned)a.parts);
+    const dim3 grid(a.N, a.parts);
     const bool ent = a.entropy != nullptr, top = a.K > 0;
     if (ent && top) hipLaunchKernelGGL((token_logprobs_kernel<T, true, true>), grid, dim3(kThr), 0, st, a);
     else if (ent) hipLaunchKernelGGL((token_logprobs_kernel<T, true, false>), grid, dim3(kThr), 0, st, a);
