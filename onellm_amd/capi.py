@@ -257,27 +257,37 @@ def topk_sample(topk_id, topk_val, output_id, seqlen, is_finished, seed, end_id,
 
 # ---------------------------------------------------------------- serving from a paged key-value cache
 
-def _same_device(*tensors):
-    """The calls below launch on the current device's stream: everything they are handed has to live there."""
+def _launch(what, ints, tensors):
+    """(device pointers of `tensors` (None: NULL), raw stream of the current device).  Everything has to be contiguous and live on
+    the current device, whose current stream the call is queued on; `ints` besides has to be int32."""
     import torch
-    here = torch.device("cuda", torch.cuda.current_device())
+    here = torch.cuda.current_device()
+    ptrs = []
     for t in tensors:
-        if t is not None and t.device != here:
-            raise ValueError(f"tensor on {t.device}, but the current device is {here}")
-
-
-def _int32(*tensors):
-    import torch
-    for t in tensors:
+        if t is None:
+            ptrs.append(None)
+            continue
+        if t.get_device() != here:
+            raise ValueError(f"{what}: tensor on {t.device}, but the current device is cuda:{here}")
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: contiguous tensors expected")
+        ptrs.append(t.data_ptr())
+    for t in ints:
         if t is not None and t.dtype != torch.int32:
-            raise TypeError(f"int32 tensor expected, not {t.dtype}")
+            raise TypeError(f"{what}: int32 tensor expected, not {t.dtype}")
+    return ptrs, torch._C._cuda_getCurrentRawStream(here)
 
 
 def _rows(t, what):
     """(pointer, token stride) of a [tokens, heads, D] tensor whose tokens may be a stride apart"""
-    if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
+    import torch
+    tokens, heads, d = t.shape
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or s1 != d:
         raise ValueError(f"{what}: [tokens, heads, D] with contiguous heads expected")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * t.shape[2])
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{what}: tensor on {t.device}, not on the current device")
+    return t.data_ptr(), s0 if tokens > 1 else max(s0, heads * d)
 
 
 def _pages(k_pages, v_pages, block_table, dtype):
@@ -305,14 +315,13 @@ def paged_qkv_store(q_out, k_pages, v_pages, qkv, bias, cu_tokens, history_lengt
         raise ValueError("q_out [tokens, Hq, D] of qkv's type and the pages' head size expected")
     if bias is not None and (bias.numel() != heads * D or bias.dtype != qkv.dtype):
         raise ValueError("bias [(Hq+2Hkv)*D] of qkv's type expected")
-    _same_device(q_out, k_pages, v_pages, qkv, bias, cu_tokens, history_length, block_table)
-    _int32(cu_tokens, history_length, block_table)
     qp, qs = _rows(q_out, "q_out")
     if q_out.data_ptr() == qkv.data_ptr() and tokens == 1:
         qs = heads * D
-    _check(lib().onellm_paged_qkv_store(_dt(qkv), qp, qs, _ptr(k_pages), _ptr(v_pages), _ptr(qkv), _ptr(bias), _ptr(cu_tokens),
-                                        _ptr(history_length), _ptr(block_table), B, tokens, Hq, Hkv, D, page_size, num_pages,
-                                        block_table.shape[1], layer, L, rotary_dim, rope_base, _stream()), "onellm_paged_qkv_store")
+    (kp, vp, xp, bp, cp, hp, tp), stream = _launch("paged_qkv_store", (cu_tokens, history_length, block_table),
+                                                   (k_pages, v_pages, qkv, bias, cu_tokens, history_length, block_table))
+    _check(lib().onellm_paged_qkv_store(_dt(qkv), qp, qs, kp, vp, xp, bp, cp, hp, tp, B, tokens, Hq, Hkv, D, page_size, num_pages,
+                                        block_table.shape[1], layer, L, rotary_dim, rope_base, stream), "onellm_paged_qkv_store")
     return q_out
 
 
@@ -329,17 +338,16 @@ def paged_prompt_attn(q, k_pages, v_pages, out, cu_tokens, history_length, block
     B = _packed(cu_tokens, history_length, block_table)
     if out.shape != q.shape or Dc != D or out.dtype != q.dtype:
         raise ValueError("out like q and the pages' head size expected")
-    _same_device(q, k_pages, v_pages, out, cu_tokens, history_length, block_table, workspace)
-    _int32(cu_tokens, history_length, block_table)
     if workspace is None:
         workspace = torch.empty(paged_prompt_attn_workspace_bytes(B, tokens, Hq, Hkv, D, int(max_rows)), dtype=torch.uint8,
                                 device=q.device)
     qp, qs = _rows(q, "q")
     op, os_ = _rows(out, "out")
-    _check(lib().onellm_paged_prompt_attn(_dt(q), qp, qs, _ptr(k_pages), _ptr(v_pages), op, os_, _ptr(cu_tokens),
-                                          _ptr(history_length), _ptr(block_table), B, tokens, Hq, Hkv, D, page_size, num_pages,
-                                          block_table.shape[1], layer, L, int(max_rows), _ptr(workspace), workspace.numel(),
-                                          _stream()), "onellm_paged_prompt_attn")
+    (kp, vp, cp, hp, tp, wp), stream = _launch("paged_prompt_attn", (cu_tokens, history_length, block_table),
+                                               (k_pages, v_pages, cu_tokens, history_length, block_table, workspace))
+    _check(lib().onellm_paged_prompt_attn(_dt(q), qp, qs, kp, vp, op, os_, cp, hp, tp, B, tokens, Hq, Hkv, D, page_size, num_pages,
+                                          block_table.shape[1], layer, L, int(max_rows), wp, workspace.numel(), stream),
+           "onellm_paged_prompt_attn")
     return out
 
 
@@ -359,15 +367,14 @@ def paged_decode_attn(qkv, bias, k_pages, v_pages, out, block_table, t_dev, max_
         raise ValueError("out [B, Hq, D] of qkv's type, t_dev [B], block_table [B, max_pages] and the pages' head size expected")
     if bias is not None and (bias.numel() != heads * D or bias.dtype != qkv.dtype):
         raise ValueError("bias [(Hq+2Hkv)*D] of qkv's type expected")
-    _same_device(qkv, bias, k_pages, v_pages, out, block_table, t_dev, workspace)
-    _int32(block_table, t_dev)
     if workspace is None:
         workspace = torch.empty(paged_decode_attn_workspace_bytes(B, Hq, Hkv, D, int(max_t)), dtype=torch.uint8, device=qkv.device)
         flags &= ~ATTN_ZEROED_WORKSPACE
-    _check(lib().onellm_paged_decode_attn(_dt(qkv), _ptr(qkv), _ptr(bias), _ptr(k_pages), _ptr(v_pages), _ptr(out),
-                                          _ptr(block_table), _ptr(t_dev), B, Hq, Hkv, D, page_size, num_pages,
-                                          block_table.shape[1], layer, L, int(max_t), rotary_dim, rope_base, flags,
-                                          _ptr(workspace), workspace.numel(), _stream()), "onellm_paged_decode_attn")
+    (xp, bp, kp, vp, op, tp, np_, wp), stream = _launch("paged_decode_attn", (block_table, t_dev),
+                                                        (qkv, bias, k_pages, v_pages, out, block_table, t_dev, workspace))
+    _check(lib().onellm_paged_decode_attn(_dt(qkv), xp, bp, kp, vp, op, tp, np_, B, Hq, Hkv, D, page_size, num_pages,
+                                          block_table.shape[1], layer, L, int(max_t), rotary_dim, rope_base, flags, wp,
+                                          workspace.numel(), stream), "onellm_paged_decode_attn")
     return out
 
 
@@ -391,11 +398,12 @@ def token_logprobs(logits, targets, K, logprob, entropy, top_ids, top_logprobs, 
         workspace = torch.empty(token_logprobs_workspace_bytes(N, V, K), dtype=torch.uint8, device=logits.device)
     if not K:
         top_ids = top_logprobs = None
-    _same_device(logits, targets, logprob, entropy, top_ids, top_logprobs, workspace)
-    _int32(targets, top_ids)
-    _check(lib().onellm_token_logprobs(_dt(logits), logits.data_ptr(), logits.stride(0) if N > 1 else max(V, logits.stride(0)),
-                                       _ptr(targets), N, V, K, _ptr(logprob), _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs),
-                                       _ptr(workspace), workspace.numel(), _stream()), "onellm_token_logprobs")
+    (tp, lp, ep, ip, vp, wp), stream = _launch("token_logprobs", (targets, top_ids),
+                                               (targets, logprob, entropy, top_ids, top_logprobs, workspace))
+    if logits.get_device() != workspace.get_device():
+        raise ValueError(f"token_logprobs: logits on {logits.device}, not on the current device")
+    _check(lib().onellm_token_logprobs(_dt(logits), logits.data_ptr(), logits.stride(0) if N > 1 else max(V, logits.stride(0)), tp, N, V,
+                                       K, lp, ep, ip, vp, wp, workspace.numel(), stream), "onellm_token_logprobs")
     return logprob, entropy, top_ids, top_logprobs
 
 

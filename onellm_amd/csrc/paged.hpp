@@ -48,17 +48,21 @@ __device__ __forceinline__ size_t paged_offset(const PagedCache& c, int page, in
 }
 
 // Rotary tables in turns per position: the angle of pair i at position p is p * f[i] turns.  The product and its reduction
-// to a fraction of a turn are done in 64 bits (error below 2^-52 of p * f, i.e. below 1e-9 rad at position 2^22), so the
+// to a fraction of a turn are done in 64 bits (off by at most 3e-14 of p * f, 2e-9 rad at position 65536), so the
 // rotation of a far position is as exact as that of a near one; p / base^(2i/dim) rounded to 32 bits would be off by
 // up to 2^-24 of the angle, 4e-3 rad at position 65536.
 struct RopeTurns { double f[kPagedMaxD / 2]; };
 
+// (one power per call, the rest by multiplication: 2^-52 relative per pair, 1e-14 at the last one)
 inline void fill_rope_turns(RopeTurns& rt, int D, int rotary_dim, float base)
 {
     constexpr double kTwoPi = 6.283185307179586476925286766559;
-    for (int i = 0; i < kPagedMaxD / 2; ++i) rt.f[i] = 0.0;
-    for (int i = 0; 2 * i < rotary_dim && 2 * i + 1 < D; ++i)
-        rt.f[i] = pow((double)base, -(double)(2 * i) / (double)rotary_dim) / kTwoPi;
+    const double step = rotary_dim > 0 ? pow((double)base, -2.0 / (double)rotary_dim) : 0.0;
+    double f = 1.0 / kTwoPi;
+    for (int i = 0; i < kPagedMaxD / 2; ++i) {
+        rt.f[i] = 2 * i < rotary_dim && 2 * i + 1 < D ? f : 0.0;
+        f *= step;
+    }
 }
 
 __device__ __forceinline__ void rope_sincos(int pos, double turns_per_pos, float& s, float& c)
@@ -105,19 +109,6 @@ inline PagedCache make_paged(const int* block_table, int max_pages, int num_page
     c.D = D;
     c.slab = (size_t)layer * num_pages * Hkv * page_size * D;
     return c;
-}
-
-// Which of the packed sequences holds token `tok`: cu[b] <= tok < cu[b + 1].  Every lane of the wave calls it with the
-// same token; 64 sequences are looked at per step, all loads of a step at once.  B when it lies behind the last one.
-__device__ __forceinline__ int sequence_of(const int* cu, int B, int tok)
-{
-    const int lane = threadIdx.x & (kWave - 1);
-    int n = 0;
-    for (int c = 0; c < B; c += kWave) {
-        const bool before = c + lane < B && cu[c + lane + 1] <= tok;
-        n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
-    }
-    return n;
 }
 
 }  // namespace onellm
