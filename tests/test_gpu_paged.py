@@ -468,3 +468,38 @@ def test_decode_agrees_with_the_contiguous_cache(capi, dev):
     flat = torch.empty(3, 8 * 128, dtype=F16, device=dev)
     capi.decode_attn(c.qkv, c.bias, kc, vc, flat, 8, 700, 128, 10000.0, rope_pos_offset=-1)
     torch.testing.assert_close(out.view(3, -1), flat, rtol=1e-2, atol=2e-3)
+
+
+# ---------------------------------------------------------------- what the Python bindings refuse
+
+def test_bindings_refuse_other_devices_types_and_layouts(capi, dev):
+    c = pm.Case(F16, [20, 9], [0, 33], 4, 2, 64, 16, seed=45)
+    out = torch.empty_like(c.q)
+    good = dict(q=c.q, kp=c.kp, vp=c.vp, out=out, cu=c.cu, hist=c.hist, table=c.table)
+
+    def prompt(**kw):
+        a = dict(good, **kw)
+        capi.paged_prompt_attn(a["q"], a["kp"], a["vp"], a["out"], a["cu"], a["hist"], a["table"], c.max_rows)
+
+    prompt()
+    for name in good:
+        with pytest.raises(ValueError):
+            prompt(**{name: good[name].cpu()})
+    for name in ("cu", "hist", "table"):
+        with pytest.raises(TypeError):
+            prompt(**{name: good[name].long()})
+    for bad in (dict(q=c.q.float()), dict(out=out.float()), dict(out=out[:, :2]), dict(kp=c.kp[0]), dict(vp=c.vp.float()), dict(cu=c.cu[:-1]),
+                dict(hist=c.hist[:1]), dict(table=c.table[:, ::2]), dict(q=c.q.transpose(1, 2).contiguous().transpose(1, 2))):
+        with pytest.raises((ValueError, TypeError)):
+            prompt(**bad)
+    with pytest.raises(ValueError):
+        capi.paged_qkv_store(out, c.kp, c.vp, c.qkv.cpu(), c.bias, c.cu, c.hist, c.table, 64, 10000.0)
+    with pytest.raises(ValueError):
+        capi.paged_qkv_store(out, c.kp, c.vp, c.qkv, c.bias[:-1], c.cu, c.hist, c.table, 64, 10000.0)
+    with pytest.raises(capi.OnellmError):
+        capi.paged_qkv_store(out, c.kp, c.vp, c.qkv, c.bias, c.cu, c.hist, c.table, 63, 10000.0)
+    t = torch.tensor([5, 5], dtype=torch.int32, device=dev)
+    for bad in (dict(t=t.cpu()), dict(t=t[:1]), dict(out=out[:1])):
+        with pytest.raises(ValueError):
+            capi.paged_decode_attn(c.qkv[:2].contiguous(), c.bias, c.kp, c.vp, bad.get("out", out[:2]), c.table, bad.get("t", t), 64, 64, 10000.0)
+    torch.cuda.synchronize()
