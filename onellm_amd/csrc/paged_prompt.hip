@@ -248,22 +248,28 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
     };
     // Masked steps: a NaN or an infinity in a V row would reach rows that do not see it (0 * NaN), so every thread
     // first replaces those among the pieces it brought by zeros; the rows that do see them get them behind the loop.
+    // (found by their exponent bits: adding one to an exponent of all ones carries into the sign's place)
     auto clean = [&](char* vb) __attribute__((always_inline)) {
-#pragma unroll 1
-        for (int i = 0; i < LD; ++i) {
-            Vec16<T>* at = reinterpret_cast<Vec16<T>*>(vb + (i * kThreads + tid) * 16);
-            Vec16<T> v = *at;
-            bool odd = false;
+        constexpr unsigned EXP = S::kHalf ? 0x7C007C00u : 0x7F800000u, ONE = S::kHalf ? 0x04000400u : 0x00800000u;
+        constexpr unsigned CARRY = S::kHalf ? 0x80008000u : 0x80000000u;
+        u32x4 v[LD];
+        unsigned carry = 0;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const bool fin = __builtin_fabsf(v.get(e)) < INFINITY;
-                odd = odd || !fin;
-                v.set(e, fin ? v.get(e) : 0.f);
+        for (int i = 0; i < LD; ++i) {
+            v[i] = *reinterpret_cast<const u32x4*>(vb + (i * kThreads + tid) * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) carry |= (v[i][e] & EXP) + ONE;
+        }
+        if (__builtin_amdgcn_ballot_w64((carry & CARRY) != 0)) {
+#pragma unroll 1
+            for (int i = 0; i < LD; ++i) {
+                Vec16<T>* at = reinterpret_cast<Vec16<T>*>(vb + (i * kThreads + tid) * 16);
+                Vec16<T> x = *at;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) x.set(e, __builtin_fabsf(x.get(e)) < INFINITY ? x.get(e) : 0.f);
+                *at = x;
             }
-            if (odd) {
-                *at = v;
-                s_odd = 1;
-            }
+            s_odd = 1;
         }
     };
 
