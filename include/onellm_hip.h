@@ -284,8 +284,8 @@ int onellm_topk_sample(const int* topk_id, const float* topk_val, int* output_id
  * may be shared between sequences as long as no call writes a shared one.  An entry outside [0, num_pages) - and any
  * row past max_pages * page_size - is "no page": its rows are neither read nor written and take no part in any sum.
  * D <= 256 and a whole number of 16-byte pieces (a multiple of 8 in fp16, of 4 in fp32); all buffers 16-byte aligned;
- * token strides (in elements) whole 16-byte pieces; B <= 65535, Hq <= 4096, max_pages * page_size < 2^30.  Anything else is
- * ONELLM_EUNSUPPORTED.
+ * token strides (in elements) whole 16-byte pieces; B <= 65535, Hq <= 4096, max_pages * page_size < 2^30, token_num <= 2^28 and
+ * token_num * Hq < 2^30.  Anything else is ONELLM_EUNSUPPORTED.
  * Packed tokens: sequence b owns tokens cu_tokens[b] .. cu_tokens[b + 1] - 1 (device int32[B + 1], ascending, inside
  * [0, token_num]; sequences may be empty) and had history_length[b] rows before them (device int32[B]); token i of a
  * sequence sits at position history_length[b] + i.  Tokens of no sequence, and those of a sequence with a negative history, are left

@@ -392,7 +392,7 @@ def token_logprobs(logits, targets, K, logprob, entropy, top_ids, top_logprobs, 
     for t, shape in ((logprob, (N,)), (entropy, (N,)), (top_logprobs if K else None, (N, K))):
         if t is not None and (t.shape != shape or t.dtype != torch.float32):
             raise ValueError(f"fp32 output of shape {shape} expected")
-    if K and top_ids.shape != (N, K) or targets is not None and targets.numel() != N:
+    if K and (top_ids is None or top_logprobs is None or top_ids.shape != (N, K)) or targets is not None and targets.numel() != N:
         raise ValueError("top_ids [N, K] and targets [N] expected")
     if workspace is None:
         workspace = torch.empty(token_logprobs_workspace_bytes(N, V, K), dtype=torch.uint8, device=logits.device)

@@ -144,6 +144,7 @@ extern "C" int onellm_paged_qkv_store(int dtype, void* q_out, long q_stride, voi
     const int vec = dtype == ONELLM_FP16 ? 8 : 4, QKVH = Hq + 2 * Hkv;
     const size_t elt = 16 / vec;
     if (q_stride < (long)Hq * D) return ONELLM_EINVAL;
+    if (token_num > 1 << 28) return ONELLM_EUNSUPPORTED;     // (token numbers are counted up past the last one in 32 bits)
     if (!aligned16(q_out) || !aligned16(qkv) || (qkv_bias && !aligned16(qkv_bias)) || q_stride % vec != 0) return ONELLM_EUNSUPPORTED;
     // q_out may be qkv itself, q written over its own heads; any other overlap would be read after it was written
     const char *o0 = static_cast<const char*>(q_out), *i0 = static_cast<const char*>(qkv);

@@ -67,7 +67,7 @@ def test_geometry(capi, call, kw, code):
     (dict(q_stride=516), "EUNSUPPORTED"), (dict(q_out=FAKE + 8), "EUNSUPPORTED"), (dict(qkv=2 * FAKE + 4), "EUNSUPPORTED"), (dict(bias=FAKE + 2), "EUNSUPPORTED"),
     # q over a part of qkv that is not its own place
     (dict(qkv=FAKE), "EINVAL"), (dict(qkv=FAKE, q_stride=1032), "EINVAL"), (dict(qkv=FAKE + 1024, q_stride=1024), "EINVAL"),
-    (dict(q_out=2 * FAKE + 3 * 8 * 128 * 2 - 16), "EINVAL"),
+    (dict(q_out=2 * FAKE + 3 * 8 * 128 * 2 - 16), "EINVAL"), (dict(tokens=2 ** 28 + 1), "EUNSUPPORTED"), (dict(tokens=2 ** 31 - 1), "EUNSUPPORTED"),
 ])
 def test_store_refusals(capi, kw, code):
     assert store(capi, **kw) == getattr(capi, code)
