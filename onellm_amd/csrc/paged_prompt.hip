@@ -57,18 +57,20 @@ __device__ __forceinline__ bool locate_tile(const PromptArgs& a, int index, Tile
         int b = c + lane, first = 0, len = 0, hist = 0, n = 0;
         if (b < a.B) {
             first = max(a.cu[b], 0);
-            len = min(a.cu[b + 1], a.token_num) - first;
+            len = min(max(a.cu[b + 1], 0), a.token_num) - first;
             hist = a.hist[b];
             if (len > 0 && hist >= 0) n = (len * a.G + kRowsPerTile - 1) / kRowsPerTile;
             hist = min(hist, 1 << 30);              // (past every table: all its rows are seen)
         }
-        const int rows = n > 0 ? hist + len : -1;
-        int rank = 0;                               // sequences with more rows (or as many, and before this one)
-        for (int j = 0; j < min(a.B - c, kWave); ++j) {
-            const int other = __builtin_amdgcn_readlane(rows, j);
-            rank += other > rows || (other == rows && j < lane) ? 1 : 0;
+        // rank by rows, no two alike (beyond 2^25 rows the order no longer matters)
+        const int key = n > 0 ? min(hist + len, (1 << 25) - 1) * kWave + (kWave - 1 - lane) : -1 - lane;
+        int rank = 0;
+        for (int j0 = 0; j0 < kWave; j0 += 16) {
+            if (c + j0 >= a.B) break;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) rank += __builtin_amdgcn_readlane(key, j0 + j) > key ? 1 : 0;
         }
-        if (b >= a.B) rank = lane;
+        if (b >= a.B) rank = lane;                  // (their keys are below all others and rank among themselves)
         b = __builtin_amdgcn_ds_permute(rank * 4, b);
         first = __builtin_amdgcn_ds_permute(rank * 4, first);
         len = __builtin_amdgcn_ds_permute(rank * 4, len);
