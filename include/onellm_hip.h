@@ -284,8 +284,8 @@ int onellm_topk_sample(const int* topk_id, const float* topk_val, int* output_id
  * may be shared between sequences as long as no call writes a shared one.  An entry outside [0, num_pages) - and any
  * row past max_pages * page_size - is "no page": its rows are neither read nor written and take no part in any sum.
  * D <= 256 and a whole number of 16-byte pieces (a multiple of 8 in fp16, of 4 in fp32); all buffers 16-byte aligned;
- * token strides (in elements) whole 16-byte pieces; B <= 65535, Hq <= 4096, max_pages * page_size < 2^30, token_num <= 2^28 and
- * token_num * Hq < 2^30.  Anything else is ONELLM_EUNSUPPORTED.
+ * token strides (in elements) whole 16-byte pieces; B <= 65535, Hq <= 4096, max_pages * page_size < 2^30, token_num <= 2^25;
+ * anything else is ONELLM_EUNSUPPORTED.
  * Packed tokens: sequence b owns tokens cu_tokens[b] .. cu_tokens[b + 1] - 1 (device int32[B + 1], ascending, inside
  * [0, token_num]; sequences may be empty) and had history_length[b] rows before them (device int32[B]); token i of a
  * sequence sits at position history_length[b] + i.  Tokens of no sequence, and those of a sequence with a negative history, are left
@@ -311,7 +311,9 @@ int onellm_paged_qkv_store(int dtype, void* q_out, long q_stride, void* k_pages,
  * Causal attention of packed tokens over the paged cache, which holds their own rows already (onellm_paged_qkv_store):
  *   out[i] = sum_j softmax_j(q[i] . k[j] / sqrt(D)) v[j]   over the rows j <= history_length[b] + i that have a page
  * for all Hq heads, kv head h / (Hq / Hkv).  A token that sees no row gets zeros.  q, out: token i at q + i * q_stride,
- * out + i * out_stride elements; out may be q.
+ * out + i * out_stride elements; out may be q with the same
+ * stride, any other shared element is ONELLM_EINVAL (rows between each other's are fine).  token_num * Hq < 2^30 and
+ * token_num * (Hq / Hkv) / 128 + min(B, token_num) <= 65535 (two million tokens of four heads per kv head): else ONELLM_EUNSUPPORTED.
  *   max_rows   upper bound of every sequence's history + tokens; where few tokens meet many rows it sizes the cut of the
  *              rows into pieces (a longer sequence is still attended in full, slower)
  *   workspace  onellm_paged_prompt_attn_workspace_bytes() bytes, 256-byte aligned, contents irrelevant; calls that share one
@@ -329,7 +331,7 @@ size_t onellm_paged_prompt_attn_workspace_bytes(int B, int token_num, int Hq, in
 /*
  * Decode attention for ONE new token per sequence over the paged cache: onellm_decode_attn's step (QKV bias, rotary position,
  * the new k and v row into the cache, attention over the sequence's rows and the new one) with the rows in pages.
- *   qkv [B, Hq + 2 Hkv, D], qkv_bias as in onellm_decode_attn (may be NULL); out [B, Hq, D]
+ *   qkv [B, Hq + 2 Hkv, D], qkv_bias as in onellm_decode_attn (may be NULL); out [B, Hq, D], no part of qkv
  *   t_dev device int32[B]: attended positions including the new token, which sits at position t - 1; a sequence whose length
  *         lies outside [1, min(max_t, max_pages * page_size)] is left alone, out row and cache included
  *   max_t upper bound of the lengths
@@ -359,7 +361,7 @@ size_t onellm_paged_decode_attn_workspace_bytes(int B, int Hq, int Hkv, int D, i
  *   top_ids, top_logprobs [N, K]: the K largest logits, larger value first, equal values: smaller token first, and x - lse
  * logits: row n at logits + n * ld elements (ld >= V), fp16 or fp32, any alignment; targets device int32[N]; outputs fp32 / int32.
  * logprob (with targets), entropy may be NULL, K may be 0 (then top_ids, top_logprobs are not read); 0 <= K <= 32, V <= 2^28,
- * N <= 2^26.
+ * N <= 2^23.
  * A logit of -inf (a banned token) has no probability and is never among the top; slots left over hold id -1 and -inf.  A row
  * of nothing but -inf: logprob -inf, entropy 0.  A NaN or +inf logit makes the row's logprob and entropy NaN; NaNs are never among the top.
  * workspace: onellm_token_logprobs_workspace_bytes() bytes, 16-byte aligned, contents irrelevant; calls that share one must not overlap.

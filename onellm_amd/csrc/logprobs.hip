@@ -467,7 +467,7 @@ extern "C" int onellm_token_logprobs(int dtype, const void* logits, long ld, con
     if (!logits || (logprob && !targets) || (K > 0 && (!top_ids || !top_logprobs))) return ONELLM_EINVAL;
     const int elt = dtype == ONELLM_FP16 ? 2 : 4;
     if (reinterpret_cast<uintptr_t>(logits) % elt != 0) return ONELLM_EINVAL;
-    if (V > (1 << 28) || N > (1 << 26)) return ONELLM_EUNSUPPORTED;
+    if (V > (1 << 28) || N > (1 << 23)) return ONELLM_EUNSUPPORTED;
     const int step = kThr * kPieces * (16 / elt);
     LogprobArgs a;
     a.logits = logits;

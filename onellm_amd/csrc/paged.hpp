@@ -111,4 +111,18 @@ inline PagedCache make_paged(const int* block_table, int max_pages, int num_page
     return c;
 }
 
+// Whether n rows of x_len elements and n of y_len, x_stride and y_stride elements apart, share memory.  Rows of one stride may lie
+// between each other's.
+inline bool rows_overlap(const void* x, long x_stride, long x_len, const void* y, long y_stride, long y_len, long n, size_t elt)
+{
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), y0 = reinterpret_cast<uintptr_t>(y);
+    const uintptr_t x1 = x0 + ((n - 1) * x_stride + x_len) * elt, y1 = y0 + ((n - 1) * y_stride + y_len) * elt;
+    if (x1 <= y0 || y1 <= x0) return false;
+    if (n == 1 || x_stride != y_stride) return true;
+    // a row of y starts d bytes behind one of x, the next one of x a stride behind that
+    const uintptr_t stride = x_stride * elt;
+    const uintptr_t d = x0 <= y0 ? (y0 - x0) % stride : (stride - (x0 - y0) % stride) % stride;
+    return d < x_len * elt || stride - d < y_len * elt;
+}
+
 }  // namespace onellm

@@ -594,6 +594,7 @@ extern "C" int onellm_paged_decode_attn(int dtype, const void* qkv, const void* 
         if (a.item_rows >= 1 << 20) return ONELLM_EUNSUPPORTED;
         a.item_rows *= 2;
     }
+    if (rows_overlap(qkv, 0, (long)B * (Hq + 2 * Hkv) * D, out, 0, (long)B * Hq * D, 1, (size_t)(row_bytes / D))) return ONELLM_EINVAL;
     p.cache = make_paged(block_table, max_pages, num_pages, page_size, Hkv, D, layer);
     p.qkv = qkv;
     p.bias = qkv_bias;

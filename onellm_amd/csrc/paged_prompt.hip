@@ -633,6 +633,8 @@ extern "C" int onellm_paged_prompt_attn(int dtype, const void* q, long q_stride,
     const int G = Hq / Hkv;
     const long tiles = tiles_bound(B, token_num, G);
     if ((long)token_num * Hq > 0x3FFFFFFFL || tiles > 65535) return ONELLM_EUNSUPPORTED;
+    const bool in_place = q == out && (q_stride == out_stride || token_num == 1);
+    if (!in_place && rows_overlap(q, q_stride, (long)Hq * D, out, out_stride, (long)Hq * D, token_num, 16 / vec)) return ONELLM_EINVAL;
     PromptArgs a;
     a.q = q;
     a.k_pages = k_pages;

@@ -76,7 +76,7 @@ void paged_qkv_store_kernel(const StoreArgs a, const RopeTurns rt)
     }
     // behind the last sequence, or a sequence that is left alone
     if (!active || b < 0 || tok < first || hist < 0) return;
-    const long long far = (long long)hist + (tok - first);
+    const long long far = (long long)hist + ((long long)tok - first);
     // a position past what the table can hold has no page; its angle is still that of the position
     const int pos = far > 0x7FFFFFFF ? 0x7FFFFFFF : (int)far;
     const int page = page_of(a.cache, a.cache.table + (size_t)b * a.cache.max_pages, pos);
@@ -144,7 +144,7 @@ extern "C" int onellm_paged_qkv_store(int dtype, void* q_out, long q_stride, voi
     const int vec = dtype == ONELLM_FP16 ? 8 : 4, QKVH = Hq + 2 * Hkv;
     const size_t elt = 16 / vec;
     if (q_stride < (long)Hq * D) return ONELLM_EINVAL;
-    if (token_num > 1 << 28) return ONELLM_EUNSUPPORTED;     // (token numbers are counted up past the last one in 32 bits)
+    if (token_num > 1 << 25) return ONELLM_EUNSUPPORTED;     // (four tokens or more per workgroup of 256: 2^31 threads, a launch takes below 2^32)
     if (!aligned16(q_out) || !aligned16(qkv) || (qkv_bias && !aligned16(qkv_bias)) || q_stride % vec != 0) return ONELLM_EUNSUPPORTED;
     // q_out may be qkv itself, q written over its own heads; any other overlap would be read after it was written
     const char *o0 = static_cast<const char*>(q_out), *i0 = static_cast<const char*>(qkv);
