@@ -589,15 +589,17 @@ long tiles_bound(int B, int token_num, int G)
 // Pieces the rows of the cache are cut into: none while the tiles alone keep the chip busy, else as many as give two workgroups
 // per compute unit, of 512 rows or more each - a second launch and the states' way through memory have to be worth it.
 // 461 tokens behind 15000..20000 rows (128 tiles, fp16): 3 / 4 / 5 / 7 pieces 197 / 181 / 194 / 190 us.
-// fp32: a tile's steps take six times as long, so the longest tile of a call ends long after the others unless it is cut:
-// four workgroups per compute unit, pieces of 128 rows (2058 tokens, 258 tiles of up to 1324 rows: uncut 89 us, two pieces 94,
-// four 76, eight 82).
-int split_of(int dtype, long tiles, int Hkv, int max_rows)
+// fp32: a tile's steps take six times as long, so the longest tile of a call ends long after the others unless it is cut: three
+// workgroups per compute unit (two where heads of more than 128 leave room for one at a time), pieces of 128 rows or more.
+// Pieces 1 / 2 / 3 / 4 / 8: 2058 tokens in 8 sequences (258 workgroups) 100 / 85 / 63 / 74 / 87 us, 2048 tokens (520) 384 / 328 / 322 / 345 / 430,
+// 1000 (264) 138 / 118 / 115 / 117 / 133, heads of 256: 1024 tokens (136) 288 / 174 / 143 / 142 / 194, 2048 (264) 567 / 360 / 386 / 406 / 546.
+int split_of(int dtype, long tiles, int Hkv, int D, int max_rows)
 {
     const bool half = dtype == ONELLM_FP16;
-    const long wgs = tiles * Hkv < 1 ? 1 : tiles * Hkv, target = half ? 512 : 1024;
+    const long wgs = tiles * Hkv < 1 ? 1 : tiles * Hkv;
     if (half && wgs > 256) return 1;
-    long n = (target + wgs / 2) / wgs;
+    const long target = D <= 128 ? 768 : 512;
+    long n = half ? (512 + wgs / 2) / wgs : (target + wgs - 1) / wgs;
     const long most = max_rows / (half ? 512 : 128);
     if (n > most) n = most;
     return n < 1 ? 1 : (int)n;
@@ -610,7 +612,7 @@ extern "C" size_t onellm_paged_prompt_attn_workspace_bytes(int B, int token_num,
 {
     using namespace onellm;
     if (B <= 0 || token_num <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || max_rows <= 0) return 256;
-    const int n = split_of(ONELLM_FP32, tiles_bound(B, token_num, Hq / Hkv), Hkv, max_rows);     // (fp16: never more)
+    const int n = split_of(ONELLM_FP32, tiles_bound(B, token_num, Hq / Hkv), Hkv, D, max_rows);     // (fp16: never more)
     if (n == 1) return 256;
     return (((size_t)n * token_num * Hq * (D + 2) * sizeof(float)) + 255) / 256 * 256;
 }
@@ -651,7 +653,7 @@ extern "C" int onellm_paged_prompt_attn(int dtype, const void* q, long q_stride,
     a.Hq = Hq;
     a.G = G;
     a.score_scale = 1.44269504088896340736f / sqrtf((float)D);
-    a.nsplit = split_of(dtype, tiles, Hkv, max_rows);
+    a.nsplit = split_of(dtype, tiles, Hkv, D, max_rows);
     a.part_o = nullptr;
     a.part_ml = nullptr;
     if (a.nsplit > 1) {
