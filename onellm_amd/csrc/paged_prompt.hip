@@ -612,7 +612,9 @@ extern "C" size_t onellm_paged_prompt_attn_workspace_bytes(int B, int token_num,
 {
     using namespace onellm;
     if (B <= 0 || token_num <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || max_rows <= 0) return 256;
-    const int n = split_of(ONELLM_FP32, tiles_bound(B, token_num, Hq / Hkv), Hkv, D, max_rows);     // (fp16: never more)
+    const long tiles = tiles_bound(B, token_num, Hq / Hkv);
+    const int half = split_of(ONELLM_FP16, tiles, Hkv, D, max_rows), full = split_of(ONELLM_FP32, tiles, Hkv, D, max_rows);
+    const int n = half > full ? half : full;
     if (n == 1) return 256;
     return (((size_t)n * token_num * Hq * (D + 2) * sizeof(float)) + 255) / 256 * 256;
 }
