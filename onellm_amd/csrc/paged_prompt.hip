@@ -588,16 +588,20 @@ long tiles_bound(int B, int token_num, int G)
 
 // Pieces the rows of the cache are cut into: none while the tiles alone keep the chip busy, else as many as give two workgroups
 // per compute unit, of 512 rows or more each - a second launch and the states' way through memory have to be worth it.
-// 461 tokens behind 15000..20000 rows (128 tiles, fp16): 3 / 4 / 5 / 7 pieces 197 / 181 / 194 / 190 us.
+// 461 tokens behind 15000..20000 rows (120 workgroups, fp16): 1 / 2 / 3 / 4 / 5 pieces 404 / 230 / 217 / 185 / 224 us.
+// A little more than one workgroup per compute unit, fp16: the longest end long after the others, so two pieces if the tiles' rows
+// differ much, as those of several sequences and of one without much before it do, and are many.  Uncut / two pieces: 4096 tokens of 8
+// heads on one (257 workgroups) 88 / 68 us, 6000 (376) 135 / 107, 500 + 500 + 200 tokens behind 500..3000 rows (320) 77 / 64, 8 x 150 behind
+// 100..3000 (360) 77 / 65; but 1400 tokens (352) 40 / 51, 1600 behind 6000 rows (408) 218 / 235, 1800 (456) 234 / 250.
 // fp32: a tile's steps take six times as long, so the longest tile of a call ends long after the others unless it is cut: three
 // workgroups per compute unit (two where heads of more than 128 leave room for one at a time), pieces of 128 rows or more.
 // Pieces 1 / 2 / 3 / 4 / 8: 2058 tokens in 8 sequences (258 workgroups) 100 / 85 / 63 / 74 / 87 us, 2048 tokens (520) 384 / 328 / 322 / 345 / 430,
 // 1000 (264) 138 / 118 / 115 / 117 / 133, heads of 256: 1024 tokens (136) 288 / 174 / 143 / 142 / 194, 2048 (264) 567 / 360 / 386 / 406 / 546.
-int split_of(int dtype, long tiles, int Hkv, int D, int max_rows)
+int split_of(int dtype, int B, int token_num, long tiles, int Hkv, int D, int max_rows)
 {
     const bool half = dtype == ONELLM_FP16;
     const long wgs = tiles * Hkv < 1 ? 1 : tiles * Hkv;
-    if (half && wgs > 256) return 1;
+    if (half && wgs > 256) return wgs <= 384 && max_rows >= 2048 && (B > 1 || max_rows / 2 < token_num) ? 2 : 1;
     const long target = D <= 128 ? 768 : 512;
     long n = half ? (512 + wgs / 2) / wgs : (target + wgs - 1) / wgs;
     const long most = max_rows / (half ? 512 : 128);
@@ -613,7 +617,7 @@ extern "C" size_t onellm_paged_prompt_attn_workspace_bytes(int B, int token_num,
     using namespace onellm;
     if (B <= 0 || token_num <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || max_rows <= 0) return 256;
     const long tiles = tiles_bound(B, token_num, Hq / Hkv);
-    const int half = split_of(ONELLM_FP16, tiles, Hkv, D, max_rows), full = split_of(ONELLM_FP32, tiles, Hkv, D, max_rows);
+    const int half = split_of(ONELLM_FP16, B, token_num, tiles, Hkv, D, max_rows), full = split_of(ONELLM_FP32, B, token_num, tiles, Hkv, D, max_rows);
     const int n = half > full ? half : full;
     if (n == 1) return 256;
     return (((size_t)n * token_num * Hq * (D + 2) * sizeof(float)) + 255) / 256 * 256;
@@ -655,7 +659,7 @@ extern "C" int onellm_paged_prompt_attn(int dtype, const void* q, long q_stride,
     a.Hq = Hq;
     a.G = G;
     a.score_scale = 1.44269504088896340736f / sqrtf((float)D);
-    a.nsplit = split_of(dtype, tiles, Hkv, D, max_rows);
+    a.nsplit = split_of(dtype, B, token_num, tiles, Hkv, D, max_rows);
     a.part_o = nullptr;
     a.part_ml = nullptr;
     if (a.nsplit > 1) {
