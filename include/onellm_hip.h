@@ -317,7 +317,7 @@ int onellm_paged_qkv_store(int dtype, void* q_out, long q_stride, void* k_pages,
  *   max_rows   upper bound of every sequence's history + tokens; where few tokens meet many rows it sizes the cut of the
  *              rows into pieces (a longer sequence is still attended in full, slower)
  *   workspace  onellm_paged_prompt_attn_workspace_bytes() bytes, 256-byte aligned, contents irrelevant; calls that share one
- *              must not overlap
+ *              must not overlap.  Fewer tokens may need more of it; 786432 (D + 2) + 256 bytes are enough for any call
  * Scores, statistics and sums are fp32; fp16 weights enter their product rounded to fp16.
  */
 int onellm_paged_prompt_attn(int dtype, const void* q, long q_stride, const void* k_pages, const void* v_pages,

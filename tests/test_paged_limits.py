@@ -43,3 +43,13 @@ def test_prompt_out_beside_q_is_taken(capi, kw):
 @pytest.mark.parametrize("out", [FAKE, FAKE + 2 * 8 * 128 * E - 16, FAKE - 2 * 4 * 128 * E + 16, FAKE + 1024])
 def test_decode_out_over_qkv(capi, out):
     assert decode(capi, out=out) == capi.EINVAL
+
+
+def test_prompt_workspace_never_grows_past_its_bound(capi):
+    for hkv in (1, 2, 8, 32, 40):
+        for g in (1, 3, 8):
+            for d in (8, 64, 128, 136, 256):
+                for tokens in (1, 2, 63, 64, 129, 500, 1100, 4000, 12000, 50000):
+                    for B in (1, 7, 300):
+                        n = capi.paged_prompt_attn_workspace_bytes(B, tokens, g * hkv, hkv, d, 2 ** 29)
+                        assert n <= 786432 * (d + 2) + 256, (B, tokens, g, hkv, d, n)
