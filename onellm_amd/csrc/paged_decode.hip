@@ -13,7 +13,10 @@
 // (up to 16 query heads of a kv head are one tile; fewer leave columns unused, the matrix pipe is far from busy).  K registers are
 // requested again as soon as the scores are there, V registers behind the output products: one buffer, always in flight.
 // Scores, statistics and sums are fp32.  fp16 caches: q and P are fp32 values split into an fp16 part and an fp16 remainder, both
-// multiplied, so they enter at 2^-22; fp32 caches multiply fp32 values.
+// multiplied, so they enter at 2^-22; fp32 caches multiply fp32 values.  What fp16's narrow range would take away is scaled into it by
+// powers of two: q / 4 cannot overflow, its remainder times 2^11 keeps its bits down to a q of 2^-25 (a small q in front of large keys;
+// scaling every head by its own largest component cost 2 us of set-up), weights times 2^14 (those of many rows that are 2^-25 or
+// less of the largest would else be lost from the output, not from the sum).
 #include <type_traits>
 #include "attn_schedule.hpp"
 #include "paged.hpp"
@@ -51,6 +54,7 @@ struct DecodeShape {
     static constexpr int NT = kHalf || DP <= 64 ? 2 : 1;    // tiles of 16 rows per wave and step
     static constexpr int RW = NT * 16;
     static constexpr int RPI = kWaves * RW;                 // rows per workgroup and step
+    static constexpr float LIFT = kHalf ? 14.f : 0.f;       // log2 of what weights, sums and outputs are scaled by until they are divided
     static constexpr int NKJ = DP / (4 * VEC);              // pieces of a K row per lane
     static constexpr int CG = (DP + 16 * VEC - 1) / (16 * VEC);   // groups of 16 pieces of a V row
     static constexpr int ACC = kWaves * kHeads * DP;        // floats: the waves' sums
@@ -68,7 +72,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t window(const void* p, unsigned
 
 // Statistics and sums of this workgroup's piece for four consecutive columns of a head, out of the waves' states in LDS and - in
 // the piece that owns it - the new token's row.
-template <int DP>
+template <typename S, int DP>
 __device__ __forceinline__ f32x4 join_waves(const float* st_ml, const float* acc, const float* snew, const float* sv, bool last, int g, int c,
                                             float& M, float& L)
 {
@@ -87,7 +91,7 @@ __device__ __forceinline__ f32x4 join_waves(const float* st_ml, const float* acc
         for (int e = 0; e < 4; ++e) O[e] = __builtin_fmaf(x[e], f, O[e]);
     }
     if (last) {
-        const float f = __builtin_amdgcn_exp2f(snew[g] - base);
+        const float f = __builtin_amdgcn_exp2f(snew[g] - base + S::LIFT);
         L += f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) O[e] = __builtin_fmaf(sv[c + e], f, O[e]);
@@ -188,6 +192,7 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
     const T* qkv = static_cast<const T*>(p.qkv) + (size_t)u.b * QKVH * D;
     const T* bias = static_cast<const T*>(p.bias);
     const int pos = u.t - 1, half_d = D / 2;
+    const float qscale = S::kHalf ? a.qscale * 0.25f : a.qscale;
     const int rows_new = ng + (u.is_last ? 2 : 0);            // heads of q, then k, then v
     Pair<T> nx[2], ny[2];
     int ng_[2], npair[2];
@@ -229,8 +234,8 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
                 x0 = r0;
             }
             if (g < ng) {
-                sq[g * DP + 2 * pr] = x0 * a.qscale;
-                sq[g * DP + 2 * pr + 1] = x1 * a.qscale;
+                sq[g * DP + 2 * pr] = x0 * qscale;
+                sq[g * DP + 2 * pr + 1] = x1 * qscale;
             } else {
                 const Pair<T> v{from_f32<T>(x0), from_f32<T>(x1)};
                 float* d = g == ng ? sk : sv;                 // the row as the cache holds it
@@ -246,7 +251,7 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
             float part = 0.f;
             for (int d = lane; d < D; d += kWave) part = __builtin_fmaf(sq[g * DP + d], sk[d], part);
             part = wave_sum(part);
-            if (lane == 0) snew[g] = part;
+            if (lane == 0) snew[g] = S::kHalf ? part * 4.f : part;
         }
     }
 
@@ -260,7 +265,7 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
             const float v = slot < ng && (grp + 4 * j) * VEC < D ? sq[slot * DP + (grp + 4 * j) * VEC + e] : 0.f;
             if constexpr (S::kHalf) {
                 qhi[j][e] = (_Float16)v;
-                qlo[j][e] = (_Float16)(v - (float)qhi[j][e]);
+                qlo[j][e] = (_Float16)((v - (float)qhi[j][e]) * 2048.f);
             } else {
                 qhi[j][e] = v;
             }
@@ -294,7 +299,7 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
             }
             const bool there = (n ? now.y : now.x) >= 0;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[n][r] = there && rb + n * 16 + 4 * grp + r < r1 ? s0[r] + s1[r] : -INFINITY;
+            for (int r = 0; r < 4; ++r) s[n][r] = there && rb + n * 16 + 4 * grp + r < r1 ? (S::kHalf ? __builtin_fmaf(s0[r], 4.f, s1[r] * (4.f / 2048.f)) : s0[r] + s1[r]) : -INFINITY;
         }
         issue_k(next, rb + S::RPI);
         float bm = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
@@ -316,7 +321,7 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
                     for (int r = 0; r < 4; ++r) o[cg][c][r] *= al[r];
             m = mnew;
         }
-        const float base = m == -INFINITY ? 0.f : m;
+        const float base = (m == -INFINITY ? 0.f : m) - S::LIFT;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -395,7 +400,7 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
         for (int i = tid; i < ng * nq; i += kThr) {
             const int g = i / nq, c = (i % nq) * 4;
             float M, L;
-            f32x4 O = join_waves<DP>(st_ml, scratch, snew, sv, u.is_last, g, c, M, L);
+            f32x4 O = join_waves<S, DP>(st_ml, scratch, snew, sv, u.is_last, g, c, M, L);
             const float inv = 1.f / L;                        // (the new token's row is always there)
 #pragma unroll
             for (int e = 0; e < 4; ++e) O[e] *= inv;
@@ -416,7 +421,7 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
     for (int i = tid; i < ng * nq; i += kThr) {
         const int g = i / nq, c = (i % nq) * 4;
         float M, L;
-        const f32x4 O = join_waves<DP>(st_ml, scratch, snew, sv, u.is_last, g, c, M, L);
+        const f32x4 O = join_waves<S, DP>(st_ml, scratch, snew, sv, u.is_last, g, c, M, L);
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, O), wo, (entry(wg, g) * D + c) * 4u, 0, kDevice);
         if (c == 0) {
             typedef unsigned u32x2 __attribute__((ext_vector_type(2)));

@@ -368,7 +368,9 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
                 for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
             mx = mnew;
         }
-        const float shift = mx == -INFINITY ? 0.f : mx * a.score_scale;      // (a row that has seen nothing yet)
+        // fp16 weights are taken times 2^7, the most that leaves room for those 256: ones of 2^-25 or less of the largest - many rows behind
+        // one that stands out - would else be lost from the output, not from the sum.
+        const float shift = (mx == -INFINITY ? 0.f : mx * a.score_scale) - (S::kHalf ? 7.f : 0.f);      // (-inf: a row that has seen nothing yet)
 #pragma unroll
         for (int n = 0; n < NS; ++n)
 #pragma unroll
