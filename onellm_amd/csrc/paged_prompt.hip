@@ -474,34 +474,62 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
     }
 
     l += __shfl_xor(l, 32, kWave);
-    if (!row_ok) return;
-    if (a.nsplit > 1) {
-        const size_t e = (size_t)blockIdx.y * ((size_t)a.token_num * a.Hq) + (size_t)(t.first + token) * a.Hq + head;
+    // The sums of a wave go through one of the four buffers, so that whole rows leave it, 16 bytes per lane: as the lanes
+    // hold them - 16 bytes each of 32 rows - a row's pieces reach memory apart from each other (four prompts of 1..100 tokens 10.2 us,
+    // so 9.7; eight of 1..2048 90.0 and 88.4).
+    const bool parts = a.nsplit > 1;
+    const float inv = parts ? 1.f : l == 0.f ? 0.f : 1.f / l;              // (a row that sees no key: zeros)
+    const size_t base = (size_t)blockIdx.y * ((size_t)a.token_num * a.Hq);
+    if (parts && row_ok && half == 0) {
+        const size_t e = base + (size_t)(t.first + token) * a.Hq + head;
+        a.part_ml[e * 2] = mx;
+        a.part_ml[e * 2 + 1] = l;
+    }
+    constexpr int COLS = S::TILE / (32 * 4) < DP ? S::TILE / (32 * 4) : DP;     // columns a buffer takes of 32 rows
+    __syncthreads();
+    float* rows = reinterpret_cast<float*>(wave == 0 ? k_even : wave == 1 ? v_even : wave == 2 ? k_odd : v_odd);
+    const int row_left = M - (t.m0 + wave * 32);           // rows of this wave
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+    for (int c0 = 0; c0 < DP; c0 += COLS) {
+#pragma unroll
+        for (int d = 0; d < COLS / 32; ++d)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
-                const int c = 32 * d + 8 * r4 + 4 * half;
-                if (c < D) *reinterpret_cast<f32x4*>(a.part_o + e * D + c) = f32x4{o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]};
+                const int piece = 8 * d + 2 * r4 + half;
+                const f32x16& x = o[c0 / 32 + d];
+                *reinterpret_cast<f32x4*>(rows + col * COLS + (piece ^ (col & 15)) * 4) =
+                    f32x4{x[4 * r4] * inv, x[4 * r4 + 1] * inv, x[4 * r4 + 2] * inv, x[4 * r4 + 3] * inv};
             }
-        if (half == 0) {
-            a.part_ml[e * 2] = mx;
-            a.part_ml[e * 2 + 1] = l;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (parts) {
+            constexpr int PER = COLS / 4, AT_ONCE = kWave / PER;           // lanes per row; rows at a time
+#pragma unroll
+            for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
+                const int r = r0 + lane / PER, piece = lane % PER, c = c0 + piece * 4;
+                const f32x4 x = *reinterpret_cast<const f32x4*>(rows + r * COLS + (piece ^ (r & 15)) * 4);
+                const int to = __shfl(token, r, kWave), h = __shfl(head, r, kWave);
+                if (r < row_left && c < D)
+                    // (written through: what the caches still hold when the launch ends is waited for. 512 tokens in two pieces 26.7 us, so 22.3)
+                    store16_write_through<false>(a.part_o + (base + (size_t)(t.first + to) * a.Hq + h) * D + c, x);
+            }
+        } else {
+            constexpr int PER = COLS / VEC, AT_ONCE = kWave / PER;
+#pragma unroll
+            for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
+                const int r = r0 + lane / PER, piece = lane % PER * (VEC / 4), c = c0 + piece * 4;
+                Vec16<T> y;
+#pragma unroll
+                for (int q = 0; q < VEC / 4; ++q) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(rows + r * COLS + ((piece + q) ^ (r & 15)) * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y.set(4 * q + e, x[e]);
+                }
+                const int to = __shfl(token, r, kWave), h = __shfl(head, r, kWave);
+                if (r < row_left && c < D) store16(static_cast<T*>(a.out) + (size_t)(t.first + to) * a.out_stride + (size_t)h * D + c, y);
+            }
         }
-        return;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;            // (a row that sees no key: zeros)
-    T* out = static_cast<T*>(a.out) + (size_t)(t.first + token) * a.out_stride + (size_t)head * D;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-            const int c = 32 * d + 8 * r4 + 4 * half;
-            if (c < D) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) out[c + e] = from_f32<T>(o[d][4 * r4 + e] * inv);
-            }
-        }
 }
 
 template <typename T, int DP>
@@ -588,9 +616,11 @@ long tiles_bound(int B, int token_num, int G)
     return rows / kRowsPerTile + (token_num < B ? token_num : B);
 }
 
-// Pieces the rows of the cache are cut into: none while the tiles alone keep the chip busy, else as many as give two workgroups
-// per compute unit, of 512 rows or more each - a second launch and the states' way through memory have to be worth it.
-// 461 tokens behind 15000..20000 rows (120 workgroups, fp16): 1 / 2 / 3 / 4 / 5 pieces 404 / 230 / 217 / 185 / 224 us.
+// Pieces the rows of the cache are cut into.  fp16, 256 workgroups or fewer: the longest tile takes 20 ns per row and 128 columns, so n
+// pieces save max_rows (1 - 1 / n) of those; they cost a second launch, 4 us, and each the states' way through memory twice, at 5 TB/s.
+// The n that is best so, if it gains anything, up to two workgroups per compute unit and 128 rows per piece.
+// 461 tokens behind 15000..20000 rows (120 workgroups) 1 / 2 / 3 / 4 / 5 pieces 404 / 230 / 217 / 185 / 224 us (four), 512 tokens of 32 heads
+// on 8 uncut / two 18.1 / 22.3 (uncut), 64 behind 800 uncut / three 24.2 / 18.4 (three), 1000 of 8 heads on 2 uncut / three 26.4 / 21.3 (three).
 // A little more than one workgroup per compute unit, fp16: the longest end long after the others, so two pieces if the tiles' rows
 // differ much, as those of several sequences and of one without much before it do, and are many.  Uncut / two pieces: 4096 tokens of 8
 // heads on one (257 workgroups) 88 / 68 us, 6000 (376) 135 / 107, 500 + 500 + 200 tokens behind 500..3000 rows (320) 77 / 64, 8 x 150 behind
@@ -599,15 +629,23 @@ long tiles_bound(int B, int token_num, int G)
 // workgroups per compute unit (two where heads of more than 128 leave room for one at a time), pieces of 128 rows or more.
 // Pieces 1 / 2 / 3 / 4 / 8: 2058 tokens in 8 sequences (258 workgroups) 100 / 85 / 63 / 74 / 87 us, 2048 tokens (520) 384 / 328 / 322 / 345 / 430,
 // 1000 (264) 138 / 118 / 115 / 117 / 133, heads of 256: 1024 tokens (136) 288 / 174 / 143 / 142 / 194, 2048 (264) 567 / 360 / 386 / 406 / 546.
-int split_of(int dtype, int B, int token_num, long tiles, int Hkv, int D, int max_rows)
+int split_of(int dtype, int B, int token_num, long tiles, int Hq, int Hkv, int D, int max_rows)
 {
-    const bool half = dtype == ONELLM_FP16;
-    const long wgs = tiles * Hkv < 1 ? 1 : tiles * Hkv;
-    if (half && wgs > 256) return wgs <= 384 && max_rows >= 2048 && (B > 1 || max_rows / 2 < token_num) ? 2 : 1;
-    const long target = D <= 128 ? 768 : 512;
-    long n = half ? (512 + wgs / 2) / wgs : (target + wgs - 1) / wgs;
-    const long most = max_rows / (half ? 512 : 128);
-    if (n > most) n = most;
+    const long wgs = tiles * Hkv < 1 ? 1 : tiles * Hkv, most = max_rows / 128;
+    long n;
+    if (dtype != ONELLM_FP16) {
+        const long target = D <= 128 ? 768 : 512;
+        n = (target + wgs - 1) / wgs;
+        if (n > most) n = most;
+    } else if (wgs > 256) {
+        n = wgs <= 384 && max_rows >= 2048 && (B > 1 || max_rows / 2 < token_num) ? 2 : 1;
+    } else {
+        const double whole = max_rows * 0.02 * D / 128.0, piece = 2.0 * token_num * Hq * D * 4.0 / 5e6;      // us
+        n = (512 + wgs / 2) / wgs;
+        if (n > most) n = most;
+        if (n * n * piece > whole) n = (long)(sqrt(whole / piece) + 0.5);
+        if (n > 1 && whole / n + n * piece + 4.0 >= whole) n = 1;
+    }
     return n < 1 ? 1 : (int)n;
 }
 
@@ -619,7 +657,7 @@ extern "C" size_t onellm_paged_prompt_attn_workspace_bytes(int B, int token_num,
     using namespace onellm;
     if (B <= 0 || token_num <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || max_rows <= 0) return 256;
     const long tiles = tiles_bound(B, token_num, Hq / Hkv);
-    const int half = split_of(ONELLM_FP16, B, token_num, tiles, Hkv, D, max_rows), full = split_of(ONELLM_FP32, B, token_num, tiles, Hkv, D, max_rows);
+    const int half = split_of(ONELLM_FP16, B, token_num, tiles, Hq, Hkv, D, max_rows), full = split_of(ONELLM_FP32, B, token_num, tiles, Hq, Hkv, D, max_rows);
     const int n = half > full ? half : full;
     if (n == 1) return 256;
     return (((size_t)n * token_num * Hq * (D + 2) * sizeof(float)) + 255) / 256 * 256;
@@ -661,7 +699,7 @@ extern "C" int onellm_paged_prompt_attn(int dtype, const void* q, long q_stride,
     a.Hq = Hq;
     a.G = G;
     a.score_scale = 1.44269504088896340736f / sqrtf((float)D);
-    a.nsplit = split_of(dtype, B, token_num, tiles, Hkv, D, max_rows);
+    a.nsplit = split_of(dtype, B, token_num, tiles, Hq, Hkv, D, max_rows);
     a.part_o = nullptr;
     a.part_ml = nullptr;
     if (a.nsplit > 1) {
