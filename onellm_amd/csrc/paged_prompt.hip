@@ -617,14 +617,15 @@ long tiles_bound(int B, int token_num, int G)
 }
 
 // Pieces the rows of the cache are cut into.  fp16, 256 workgroups or fewer: the longest tile takes 20 ns per row and 128 columns, so n
-// pieces save max_rows (1 - 1 / n) of those; they cost a second launch, 4 us, and each the states' way through memory twice, at 5 TB/s.
-// The n that is best so, if it gains anything, up to two workgroups per compute unit and 128 rows per piece.
+// pieces a 1 / n of that (1.45 / n where two share a compute unit); they cost a second launch, 4 us, and each the states' way through
+// memory twice, at 6 TB/s.  The n that is best so, up to two workgroups per compute unit and 128 rows per piece.
 // 461 tokens behind 15000..20000 rows (120 workgroups) 1 / 2 / 3 / 4 / 5 pieces 404 / 230 / 217 / 185 / 224 us (four), 512 tokens of 32 heads
-// on 8 uncut / two 18.1 / 22.3 (uncut), 64 behind 800 uncut / three 24.2 / 18.4 (three), 1000 of 8 heads on 2 uncut / three 26.4 / 21.3 (three).
+// on 8 uncut / two 18.1 / 22.3 (uncut), 64 behind 800 uncut / three / six 24.2 / 18.4 / 16.1 (six), 1000 of 8 heads on 2 uncut / three
+// 26.4 / 21.1 (three), 1000 of 32 on 8 behind 3000 uncut / two 92.5 / 83.8 (two), 400 behind 1000 two / five 29.5 / 33.1 (two).
 // A little more than one workgroup per compute unit, fp16: the longest end long after the others, so two pieces if the tiles' rows
-// differ much, as those of several sequences and of one without much before it do, and are many.  Uncut / two pieces: 4096 tokens of 8
+// differ much, as those of several sequences and of one with little before it do, and are many.  Uncut / two pieces: 4096 tokens of 8
 // heads on one (257 workgroups) 88 / 68 us, 6000 (376) 135 / 107, 500 + 500 + 200 tokens behind 500..3000 rows (320) 77 / 64, 8 x 150 behind
-// 100..3000 (360) 77 / 65; but 1400 tokens (352) 40 / 51, 1600 behind 6000 rows (408) 218 / 235, 1800 (456) 234 / 250.
+// 100..3000 (360) 77 / 65; but 1400 tokens (352) 40 / 51, 1100 behind 1000 rows (280) 53 / 65, 1600 behind 6000 (408) 210 / 227.
 // fp32: a tile's steps take six times as long, so the longest tile of a call ends long after the others unless it is cut: three
 // workgroups per compute unit (two where heads of more than 128 leave room for one at a time), pieces of 128 rows or more.
 // Pieces 1 / 2 / 3 / 4 / 8: 2058 tokens in 8 sequences (258 workgroups) 100 / 85 / 63 / 74 / 87 us, 2048 tokens (520) 384 / 328 / 322 / 345 / 430,
@@ -638,13 +639,22 @@ int split_of(int dtype, int B, int token_num, long tiles, int Hq, int Hkv, int D
         n = (target + wgs - 1) / wgs;
         if (n > most) n = most;
     } else if (wgs > 256) {
-        n = wgs <= 384 && max_rows >= 2048 && (B > 1 || max_rows / 2 < token_num) ? 2 : 1;
+        n = wgs <= 384 && max_rows >= 2048 && (B > 1 || max_rows / 4 * 3 < token_num) ? 2 : 1;
     } else {
-        const double whole = max_rows * 0.02 * D / 128.0, piece = 2.0 * token_num * Hq * D * 4.0 / 5e6;      // us
-        n = (512 + wgs / 2) / wgs;
-        if (n > most) n = most;
-        if (n * n * piece > whole) n = (long)(sqrt(whole / piece) + 0.5);
-        if (n > 1 && whole / n + n * piece + 4.0 >= whole) n = 1;
+        const double whole = max_rows * 0.02 * D / 128.0, piece = 2.0 * token_num * Hq * D * 4.0 / 6e6;      // us
+        double best = whole;
+        n = 1;
+        for (int two = 0; two < 2; ++two) {
+            const double sole = two ? 1.45 * whole : whole;
+            long c = two ? (512 + wgs / 2) / wgs : 256 / wgs;
+            if (c > most) c = most;
+            if (c * c * piece > sole) c = (long)(sqrt(sole / piece) + 0.5);
+            const double time = sole / c + c * piece + 4.0;
+            if (c > 1 && time < best) {
+                best = time;
+                n = c;
+            }
+        }
     }
     return n < 1 ? 1 : (int)n;
 }
