@@ -7,6 +7,7 @@
 // entropy = ln 2 (log2 Z - S / Z) - differences only, so a row of large or very negative logits loses nothing.
 // Per logit that is a multiply-add, an exponential (two issue slots), an add and for the entropy a clamp and a multiply-add; with
 // half a slot for the maximum that is 6.5 slots, 22 us for 4096 x 32000 logits on all SIMDs against 37 us to read them in fp16.
+// Measured: 55 us with entropy and the 8 best (47..50 without the list), 4.8 TB/s; 16 x 32000 fp32 and the 5 best 9.5 us, two launches.
 //
 // The K best: a wave keeps candidates in LDS as 64-bit keys (value, then lower token first).  The K-th largest of the first step's
 // 256 lane maxima, found bit by bit with ballots, is a floor below which nothing can be among the K best; the lanes that reach

@@ -3,6 +3,9 @@
 //
 //   out = sum_j softmax_j(q . k[j] / sqrt(D)) v[j]          2 flops per byte and query head: HBM-bound
 //
+// 16 x 4096 rows of 32 kv heads of 128, fp16: 163 us, 6.6 TB/s, the time of the loads alone; 32 x 1024..8192 rows of 8 heads, 32 query
+// heads: 100 us; one sequence of 900 rows: 12 us, a chain of dependent loads.
+//
 // The rows of the step are cut and dealt by the balanced schedule of attn_schedule.hpp (equal cost per workgroup whatever
 // the lengths).  A wave takes 16 or 32 rows per step straight into registers, 16 bytes per lane, through windows of 16 rows each
 // lie in one page: rows past the piece's end and rows of a page that is none arrive as zeros and are masked, so no load of

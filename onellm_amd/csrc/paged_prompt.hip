@@ -10,8 +10,14 @@
 // lane exchange per tile, and the registers it leaves are, as they stand, the B operand of O^T = V^T P^T: product i takes
 // the keys its lanes hold, and V^T's operand picks the same keys.  For fp16 that operand (a column of V over four
 // keys) comes out of the LDS transposed (ds_read_b64_tr_b16); for fp32 a product takes two keys and reads them as they are.
-// Scores, statistics and output are fp32.  fp16: P enters its product rounded to fp16 (half a step, 2^-12 relative of each
+// Scores, statistics and output are fp32.  fp16: P enters its product rounded to fp16 (half a step, 2^-11 relative of each
 // weight, averaged over the keys); the sum of the weights is taken before that rounding.
+//
+// 128 rows per workgroup: every K and V row that comes through LDS is then used for 128 products, and a wave's 32 rows of scores, output
+// and Q leave room for two workgroups on a compute unit (heads up to 128), of which one multiplies while the other takes exponentials.
+// Bound by that pair of units, not by memory: 8192 tokens of 32 heads on 8 of 128, fp16, 550 us, 1000 TFLOP/s (a library product of
+// 16384^3 reaches 1266 on the same card), matrix cores 54 % busy and the vector unit 50 %.  2058 tokens in four sequences, fp32, 16 heads on 2
+// of 64: 62 us.
 #include <type_traits>
 #include "paged.hpp"
 

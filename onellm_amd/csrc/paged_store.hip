@@ -1,6 +1,7 @@
 // Packed tokens into a paged key-value cache: QKV bias, rotary positions, q to its buffer, k and v rows to their pages.
 //
-// HBM-bound: every element is read once and written once, 2 * tokens * (Hq + 2 Hkv) * D * e bytes.
+// HBM-bound: every element is read once and written once, 2 * tokens * (Hq + 2 Hkv) * D * e bytes.  4 x 2048 tokens, 96 heads of 128,
+// fp16: 75 us, 5.4 TB/s (a plain device copy: 5.15).  4 x 8 tokens of 48 heads: 4 us, a launch and three dependent loads.
 #include "paged.hpp"
 
 namespace onellm {
