@@ -109,12 +109,14 @@ __device__ __forceinline__ void store16_stream(T* p, const Vec16<T>& v)
 // with sc1 + nt (sc1 alone: 2 %), a prefill-sized KV append 12 % faster with sc1 alone (sc1 + nt: 7 %), an in-place
 // read-modify-write stream 2 % with sc1 + nt.  Kernels that read two streams per stream written (SwiGLU, the
 // prefill transpose) are 0.5-2 % slower with either and keep the plain non-temporal store.
+// (A store of more than 8 bytes reads its data up to two wait states after it was issued; the compiler keeps that distance for its own
+// stores, but does not see into the assembly: hence the s_nop, without which the next instruction but one changed what was stored.)
 typedef float stream_f32x4 __attribute__((ext_vector_type(4)));
 template <bool NT>
 __device__ __forceinline__ void store16_write_through(void* p, stream_f32x4 v)
 {
-    if constexpr (NT) asm volatile("global_store_dwordx4 %0, %1, off sc1 nt" : : "v"(p), "v"(v) : "memory");
-    else asm volatile("global_store_dwordx4 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
+    if constexpr (NT) asm volatile("global_store_dwordx4 %0, %1, off sc1 nt\n\ts_nop 1" : : "v"(p), "v"(v) : "memory");
+    else asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" : : "v"(p), "v"(v) : "memory");
 }
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
