@@ -55,12 +55,25 @@ struct Tile {
     int m0;                    // first row of the tile: token m / G, head m % G of the group
 };
 
+// sum over the lanes up to this one
+__device__ __forceinline__ int wave_scan(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);        // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);        // lane 15 of the row before, to rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);        // lane 31, to rows 2 and 3
+    return v;
+}
+
 __device__ __forceinline__ bool locate_tile(const PromptArgs& a, int index, Tile& t)
 {
     const int lane = threadIdx.x & (kWave - 1);
     int run = 0;
     for (int c = 0; c < a.B; c += kWave) {
-        int b = c + lane, first = 0, len = 0, hist = 0, n = 0;
+        const int b = c + lane;
+        int first = 0, len = 0, hist = 0, n = 0;
         if (b < a.B) {
             first = max(a.cu[b], 0);
             len = min(max(a.cu[b + 1], 0), a.token_num) - first;
@@ -77,24 +90,17 @@ __device__ __forceinline__ bool locate_tile(const PromptArgs& a, int index, Tile
             for (int j = 0; j < 16; ++j) rank += __builtin_amdgcn_readlane(key, j0 + j) > key ? 1 : 0;
         }
         if (b >= a.B) rank = lane;                  // (their keys are below all others and rank among themselves)
-        b = __builtin_amdgcn_ds_permute(rank * 4, b);
-        first = __builtin_amdgcn_ds_permute(rank * 4, first);
-        len = __builtin_amdgcn_ds_permute(rank * 4, len);
-        hist = __builtin_amdgcn_ds_permute(rank * 4, hist);
-        n = __builtin_amdgcn_ds_permute(rank * 4, n);
-        int inc = n;
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const int up = __shfl_up(inc, o, kWave);
-            if (lane >= o) inc += up;
-        }
+        // in the order of the ranks: whose turn it is, and how many tiles there are up to its last
+        const int whose = __builtin_amdgcn_ds_permute(rank * 4, lane);
+        const int inc = wave_scan(__builtin_amdgcn_ds_permute(rank * 4, n));
         const int tot = __builtin_amdgcn_readlane(inc, kWave - 1);
         if (index < run + tot) {
             const int f = __builtin_ctzll(__builtin_amdgcn_ballot_w64(run + inc > index));
-            t.b = __builtin_amdgcn_readlane(b, f);
-            t.first = __builtin_amdgcn_readlane(first, f);
-            t.len = __builtin_amdgcn_readlane(len, f);
-            t.hist = __builtin_amdgcn_readlane(hist, f);
+            const int from = __builtin_amdgcn_readlane(whose, f);
+            t.b = c + from;
+            t.first = __builtin_amdgcn_readlane(first, from);
+            t.len = __builtin_amdgcn_readlane(len, from);
+            t.hist = __builtin_amdgcn_readlane(hist, from);
             t.m0 = (run + __builtin_amdgcn_readlane(inc, f) - 1 - index) * kRowsPerTile;
             return true;
         }
@@ -634,8 +640,8 @@ long tiles_bound(int B, int token_num, int G)
 // 100..3000 (360) 77 / 65; but 1400 tokens (352) 40 / 51, 1100 behind 1000 rows (280) 53 / 65, 1600 behind 6000 (408) 210 / 227.
 // fp32: a tile's steps take six times as long, so the longest tile of a call ends long after the others unless it is cut: three
 // workgroups per compute unit (two where heads of more than 128 leave room for one at a time), pieces of 128 rows or more.
-// Pieces 1 / 2 / 3 / 4 / 8: 2058 tokens in 8 sequences (258 workgroups) 100 / 85 / 63 / 74 / 87 us, 2048 tokens (520) 384 / 328 / 322 / 345 / 430,
-// 1000 (264) 138 / 118 / 115 / 117 / 133, heads of 256: 1024 tokens (136) 288 / 174 / 143 / 142 / 194, 2048 (264) 567 / 360 / 386 / 406 / 546.
+// Pieces 1 / 2 / 3 / 4 / 8: 2058 tokens in 4 sequences (264 workgroups) 100 / 85 / 63 / 74 / 87 us, 2048 tokens (520) 384 / 328 / 322 / 345 / 430,
+// 1000 (256) 138 / 118 / 115 / 117 / 133, heads of 256: 1024 tokens (136) 288 / 174 / 143 / 142 / 194, 2048 (264) 567 / 360 / 386 / 406 / 546.
 int split_of(int dtype, int B, int token_num, long tiles, int Hq, int Hkv, int D, int max_rows)
 {
     const long wgs = tiles * Hkv < 1 ? 1 : tiles * Hkv, most = max_rows / 128;
