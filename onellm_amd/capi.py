@@ -257,35 +257,30 @@ def topk_sample(topk_id, topk_val, output_id, seqlen, is_finished, seed, end_id,
 
 # ---------------------------------------------------------------- serving from a paged key-value cache
 
-def _launch(what, ints, tensors):
+def _launch(what, ints, tensors, here=None):
     """(device pointers of `tensors` (None: NULL), raw stream of the current device).  Everything has to be contiguous and live on
     the current device, whose current stream the call is queued on; `ints` besides has to be int32."""
     import torch
-    here = torch.cuda.current_device()
-    ptrs = []
+    if here is None:
+        here = torch.cuda.current_device()
     for t in tensors:
-        if t is None:
-            ptrs.append(None)
-            continue
-        if t.get_device() != here:
-            raise ValueError(f"{what}: tensor on {t.device}, but the current device is cuda:{here}")
-        if not t.is_contiguous():
-            raise ValueError(f"{what}: contiguous tensors expected")
-        ptrs.append(t.data_ptr())
+        if t is not None and (t.get_device() != here or not t.is_contiguous()):
+            raise ValueError(f"{what}: contiguous tensors expected" if t.get_device() == here else
+                             f"{what}: tensor on {t.device}, but the current device is cuda:{here}")
+    i32 = torch.int32
     for t in ints:
-        if t is not None and t.dtype != torch.int32:
+        if t is not None and t.dtype is not i32:
             raise TypeError(f"{what}: int32 tensor expected, not {t.dtype}")
-    return ptrs, torch._C._cuda_getCurrentRawStream(here)
+    return [None if t is None else t.data_ptr() for t in tensors], torch._C._cuda_getCurrentRawStream(here)
 
 
-def _rows(t, what):
+def _rows(t, what, here):
     """(pointer, token stride) of a [tokens, heads, D] tensor whose tokens may be a stride apart"""
-    import torch
     tokens, heads, d = t.shape
     s0, s1, s2 = t.stride()
     if s2 != 1 or s1 != d:
         raise ValueError(f"{what}: [tokens, heads, D] with contiguous heads expected")
-    if t.get_device() != torch.cuda.current_device():
+    if t.get_device() != here:
         raise ValueError(f"{what}: tensor on {t.device}, not on the current device")
     return t.data_ptr(), s0 if tokens > 1 else max(s0, heads * d)
 
@@ -307,6 +302,7 @@ def _packed(cu_tokens, history_length, block_table):
 
 def paged_qkv_store(q_out, k_pages, v_pages, qkv, bias, cu_tokens, history_length, block_table, rotary_dim, rope_base, layer=0):
     """qkv [tokens, Hq+2Hkv, D]; q_out [tokens, Hq, D] (may be qkv[:, :Hq]); pages [L, pages, Hkv, page_size, D]."""
+    import torch
     tokens, heads, D = qkv.shape
     L, num_pages, Hkv, page_size, Dc = _pages(k_pages, v_pages, block_table, qkv.dtype)
     Hq = heads - 2 * Hkv
@@ -315,11 +311,12 @@ def paged_qkv_store(q_out, k_pages, v_pages, qkv, bias, cu_tokens, history_lengt
         raise ValueError("q_out [tokens, Hq, D] of qkv's type and the pages' head size expected")
     if bias is not None and (bias.numel() != heads * D or bias.dtype != qkv.dtype):
         raise ValueError("bias [(Hq+2Hkv)*D] of qkv's type expected")
-    qp, qs = _rows(q_out, "q_out")
+    here = torch.cuda.current_device()
+    qp, qs = _rows(q_out, "q_out", here)
     if q_out.data_ptr() == qkv.data_ptr() and tokens == 1:
         qs = heads * D
     (kp, vp, xp, bp, cp, hp, tp), stream = _launch("paged_qkv_store", (cu_tokens, history_length, block_table),
-                                                   (k_pages, v_pages, qkv, bias, cu_tokens, history_length, block_table))
+                                                   (k_pages, v_pages, qkv, bias, cu_tokens, history_length, block_table), here)
     _check(lib().onellm_paged_qkv_store(_dt(qkv), qp, qs, kp, vp, xp, bp, cp, hp, tp, B, tokens, Hq, Hkv, D, page_size, num_pages,
                                         block_table.shape[1], layer, L, rotary_dim, rope_base, stream), "onellm_paged_qkv_store")
     return q_out
@@ -341,10 +338,11 @@ def paged_prompt_attn(q, k_pages, v_pages, out, cu_tokens, history_length, block
     if workspace is None:
         workspace = torch.empty(paged_prompt_attn_workspace_bytes(B, tokens, Hq, Hkv, D, int(max_rows)), dtype=torch.uint8,
                                 device=q.device)
-    qp, qs = _rows(q, "q")
-    op, os_ = _rows(out, "out")
+    here = torch.cuda.current_device()
+    qp, qs = _rows(q, "q", here)
+    op, os_ = _rows(out, "out", here)
     (kp, vp, cp, hp, tp, wp), stream = _launch("paged_prompt_attn", (cu_tokens, history_length, block_table),
-                                               (k_pages, v_pages, cu_tokens, history_length, block_table, workspace))
+                                               (k_pages, v_pages, cu_tokens, history_length, block_table, workspace), here)
     _check(lib().onellm_paged_prompt_attn(_dt(q), qp, qs, kp, vp, op, os_, cp, hp, tp, B, tokens, Hq, Hkv, D, page_size, num_pages,
                                           block_table.shape[1], layer, L, int(max_rows), wp, workspace.numel(), stream),
            "onellm_paged_prompt_attn")
