@@ -585,8 +585,9 @@ void paged_prompt_merge_kernel(const PromptArgs a)
         for (int e = 0; e < 4; ++e) O[e] *= keep;
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
-            // (a piece that saw nothing has no weight, whatever its state holds)
-            const bool on = s0 + j < a.nsplit && m[j] != -INFINITY;
+            // (a piece that saw nothing - no maximum and no sum - has no weight; one whose scores are all NaN has no maximum either, but its sum
+            // is NaN, and so is the row)
+            const bool on = s0 + j < a.nsplit && (m[j] != -INFINITY || l[j] != 0.f);
             const float w = on ? __builtin_amdgcn_exp2f((m[j] - bm) * a.score_scale) : 0.f;
             L = on ? __builtin_fmaf(l[j], w, L) : L;
 #pragma unroll
