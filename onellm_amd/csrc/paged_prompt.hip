@@ -110,6 +110,7 @@ __device__ __forceinline__ bool locate_tile(const PromptArgs& a, int index, Tile
 }
 
 constexpr unsigned kOutside = 0x7FFFFF00u;     // a byte offset no window of 16 rows reaches
+constexpr float kFar = 4096.f;
 
 template <typename T, int DP>
 struct PromptShape {
@@ -202,6 +203,7 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
     if (tid == 0) s_odd = 0;
     float mx = -INFINITY, l = 0.f;                  // of this lane's row: what weights are relative to; their sum over this lane's keys
     const float slack = 8.f / a.score_scale;
+    bool far = false;                               // a row of the wave has a reference of 2^12 or more in units of log 2
     f32x16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -370,7 +372,7 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
         bm = other_half_max(bm);
         // What the weights are taken against only follows the maximum when that has grown by 2^8 or more: weights of up to 256 lose
         // nothing (a rounding is relative), and a row's sum and output are rescaled a few times, not every few steps.
-        if (__builtin_amdgcn_ballot_w64(bm > mx + slack) != 0) {
+        if (__builtin_amdgcn_ballot_w64(bm - mx > slack) != 0) {
             const float mnew = fmaxf(mx, bm);
             const float alpha = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mx - mnew) * a.score_scale);
             l *= alpha;
@@ -379,10 +381,23 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
             mx = mnew;
+            far = __builtin_amdgcn_ballot_w64(mx != -INFINITY && __builtin_fabsf(mx * a.score_scale) >= kFar) != 0;
         }
         // fp16 weights are taken times 2^7, the most that leaves room for those 256: ones of 2^-25 or less of the largest - many rows behind
         // one that stands out - would else be lost from the output, not from the sum.
-        const float shift = (mx == -INFINITY ? 0.f : mx * a.score_scale) - (S::kHalf ? 7.f : 0.f);      // (-inf: a row that has seen nothing yet)
+        constexpr float LIFT = S::kHalf ? 7.f : 0.f;
+        const float base = mx == -INFINITY ? 0.f : mx;                     // (-inf: a row that has seen nothing yet)
+        float shift = base * a.score_scale - LIFT;
+        // Far from zero the product of base and scale is rounded by more than a weight can bear (at 2^12 by 2^-13, at 2^25 by 1 - and the
+        // weights have 2^0.99 left), so there the scores' differences come first, which are exact where they count.  (8192 tokens: in every
+        // step 590 us, behind this branch 577, without it 574)
+        if (far) {
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[n][r] -= base;
+            shift = -LIFT;
+        }
 #pragma unroll
         for (int n = 0; n < NS; ++n)
 #pragma unroll
