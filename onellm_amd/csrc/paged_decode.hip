@@ -57,7 +57,7 @@ struct DecodeShape {
     static constexpr int NT = kHalf || DP <= 64 ? 2 : 1;    // tiles of 16 rows per wave and step
     static constexpr int RW = NT * 16;
     static constexpr int RPI = kWaves * RW;                 // rows per workgroup and step
-    static constexpr float LIFT = kHalf ? 14.f : 0.f;       // log2 of what weights, sums and outputs are scaled by until they are divided
+    static constexpr float LIFT = kHalf ? 16384.f : 1.f;    // what weights, sums and outputs are scaled by until they are divided
     static constexpr int NKJ = DP / (4 * VEC);              // pieces of a K row per lane
     static constexpr int CG = (DP + 16 * VEC - 1) / (16 * VEC);   // groups of 16 pieces of a V row
     static constexpr int ACC = kWaves * kHeads * DP;        // floats: the waves' sums
@@ -94,7 +94,7 @@ __device__ __forceinline__ f32x4 join_waves(const float* st_ml, const float* acc
         for (int e = 0; e < 4; ++e) O[e] = __builtin_fmaf(x[e], f, O[e]);
     }
     if (last) {
-        const float f = __builtin_amdgcn_exp2f(snew[g] - base + S::LIFT);
+        const float f = __builtin_amdgcn_exp2f(snew[g] - base) * S::LIFT;
         L += f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) O[e] = __builtin_fmaf(sv[c + e], f, O[e]);
@@ -324,12 +324,14 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
                     for (int r = 0; r < 4; ++r) o[cg][c][r] *= al[r];
             m = mnew;
         }
-        const float base = (m == -INFINITY ? 0.f : m) - S::LIFT;
+        // (the lift is a factor, not part of the exponent: next to a score of 2^25 and more 14 would be rounded to 16, and the largest weights
+        // would leave fp16)
+        const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - base);
+                s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - base) * S::LIFT;
                 l += s[n][r];
             }
         if constexpr (S::kHalf) {
