@@ -204,6 +204,7 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
     float mx = -INFINITY, l = 0.f;                  // of this lane's row: what weights are relative to; their sum over this lane's keys
     const float slack = 8.f / a.score_scale;
     bool far = false;                               // a row of the wave has a reference of 2^12 or more in units of log 2
+    auto is_far = [&](float ref) __attribute__((always_inline)) { return ref != -INFINITY && __builtin_fabsf(ref * a.score_scale) >= kFar; };
     f32x16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -373,7 +374,7 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
         // What the weights are taken against only follows the maximum when that has grown by 2^8 or more: weights of up to 256 lose
         // nothing (a rounding is relative), and a row's sum and output are rescaled a few times, not every few steps.
         if (__builtin_amdgcn_ballot_w64(bm - mx > slack) != 0) {
-            const float mnew = fmaxf(mx, bm);
+            const float mnew = bm - mx > slack ? bm : mx;     // (each row by itself: what it gets does not hang on its neighbours)
             const float alpha = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mx - mnew) * a.score_scale);
             l *= alpha;
 #pragma unroll
@@ -381,7 +382,7 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
             mx = mnew;
-            far = __builtin_amdgcn_ballot_w64(mx != -INFINITY && __builtin_fabsf(mx * a.score_scale) >= kFar) != 0;
+            far = __builtin_amdgcn_ballot_w64(is_far(mx)) != 0;
         }
         // fp16 weights are taken times 2^7, the most that leaves room for those 256: ones of 2^-25 or less of the largest - many rows behind
         // one that stands out - would else be lost from the output, not from the sum.
@@ -392,11 +393,12 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
         // weights have 2^0.99 left), so there the scores' differences come first, which are exact where they count.  (8192 tokens: in every
         // step 590 us, behind this branch 577, without it 574)
         if (far) {
+            const float own = is_far(mx) ? mx : 0.f;
 #pragma unroll
             for (int n = 0; n < NS; ++n)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[n][r] -= base;
-            shift = -LIFT;
+                for (int r = 0; r < 16; ++r) s[n][r] -= own;
+            shift = is_far(mx) ? -LIFT : shift;
         }
 #pragma unroll
         for (int n = 0; n < NS; ++n)

@@ -49,3 +49,14 @@ def test_prompt(capi, dev, dtype, cut, a, b, growing):
         w = torch.softmax(8.0 * m[:n], dim=0)
         want[i, 0], mean[i, 0] = w @ v[:n], w @ v[:n].abs()
     within(got, want, mean, dtype, rows, float(v.abs().max()))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_prompt_rows_of_one_wave_do_not_touch_each_other(capi, dev, dtype):
+    """a token whose scores are far from zero, beside tokens whose are not: these come out bit for bit as without it"""
+    c = pm.Case(dtype, [8], [300], 1, 1, 64, 16, seed=75)
+    clean = prompt(capi, c)
+    c.q[3] *= 2.0 ** 10
+    got = prompt(capi, c)
+    others = [0, 1, 2, 4, 5, 6, 7]
+    assert torch.equal(got[others], clean[others])
