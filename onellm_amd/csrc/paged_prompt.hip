@@ -111,6 +111,7 @@ __device__ __forceinline__ bool locate_tile(const PromptArgs& a, int index, Tile
 
 constexpr unsigned kOutside = 0x7FFFFF00u;     // a byte offset no window of 16 rows reaches
 constexpr float kFar = 4096.f;
+constexpr float kLowest = -3.4028234664e38f;
 
 template <typename T, int DP>
 struct PromptShape {
@@ -503,11 +504,22 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
     }
 
     l += __shfl_xor(l, 32, kWave);
+    // (rare) No sum although there are rows up to the limit: either none of them has a page, or all scores are -inf, and then there is no
+    // distribution - NaN, unless another piece has one: its maximum is above the lowest value that stands here for "saw only -inf".
+    bool lost = false;
+    if (__builtin_amdgcn_ballot_w64(l == 0.f && limit >= k_begin) != 0) {
+#pragma unroll 1
+        for (int row = k_begin; row < k_end; row += kRowGroup) {
+            const int page = __builtin_amdgcn_readfirstlane(page_of(a.cache, table, row));
+            lost = lost || (page >= 0 && row <= limit && l == 0.f);
+        }
+        if (lost) mx = kLowest;
+    }
     // The sums of a wave go through one of the four buffers, so that whole rows leave it, 16 bytes per lane: as the lanes
     // hold them - 16 bytes each of 32 rows - a row's pieces reach memory apart from each other (four prompts of 1..100 tokens 10.2 us,
     // so 9.7; eight of 1..2048 90.0 and 88.4).
     const bool parts = a.nsplit > 1;
-    const float inv = parts ? 1.f : l == 0.f ? 0.f : 1.f / l;              // (a row that sees no key: zeros)
+    const float inv = parts ? 1.f : l == 0.f && !lost ? 0.f : 1.f / l;     // (a row that sees no key: zeros)
     const size_t base = (size_t)blockIdx.y * ((size_t)a.token_num * a.Hq);
     if (parts && row_ok && half == 0) {
         const size_t e = base + (size_t)(t.first + token) * a.Hq + head;
@@ -619,7 +631,7 @@ void paged_prompt_merge_kernel(const PromptArgs a)
         else hi = mid;
     }
     if (lo >= a.B || token < a.cu[lo] || a.hist[lo] < 0) return;
-    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const float inv = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;          // (no piece saw a row: zeros; only scores of -inf: 0 / 0)
     T* out = static_cast<T*>(a.out) + (size_t)token * a.out_stride + (size_t)head * a.cache.D + c;
 #pragma unroll
     for (int e = 0; e < 4; ++e) out[e] = from_f32<T>(O[e] * inv);
