@@ -310,7 +310,9 @@ int onellm_paged_qkv_store(int dtype, void* q_out, long q_stride, void* k_pages,
 /*
  * Causal attention of packed tokens over the paged cache, which holds their own rows already (onellm_paged_qkv_store):
  *   out[i] = sum_j softmax_j(q[i] . k[j] / sqrt(D)) v[j]   over the rows j <= history_length[b] + i that have a page
- * for all Hq heads, kv head h / (Hq / Hkv).  A token that sees no row gets zeros, one whose scores are all -inf or hold a NaN gets NaN.  q, out: token i at q + i * q_stride,
+ * for all Hq heads, kv head h / (Hq / Hkv).  A token that sees no row gets zeros, one whose scores are all -inf or hold a NaN gets NaN.
+ * NaNs and infinities in rows of V that a token sees: its component is the sum of those in the column, whatever their weights (inf or NaN); other
+ * components and tokens are as without them.  q, out: token i at q + i * q_stride,
  * out + i * out_stride elements; out may be q with the same
  * stride, any other shared element is ONELLM_EINVAL (rows between each other's are fine).  token_num * Hq < 2^30 and
  * token_num * (Hq / Hkv) / 128 + min(B, token_num) <= 65535 (two million tokens of four heads per kv head): else ONELLM_EUNSUPPORTED.

@@ -202,6 +202,7 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
     }
 
     if (tid == 0) s_odd = 0;
+    int odd_from = k_begin;
     float mx = -INFINITY, l = 0.f;                  // of this lane's row: what weights are relative to; their sum over this lane's keys
     const float slack = 8.f / a.score_scale;
     bool far = false;                               // a row of the wave has a reference of 2^12 or more in units of log 2
@@ -393,7 +394,7 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
         // Far from zero the product of base and scale is rounded by more than a weight can bear (at 2^12 by 2^-13, at 2^25 by 1 - and the
         // weights have 2^0.99 left), so there the scores' differences come first, which are exact where they count.  (8192 tokens: in every
         // step 590 us, behind this branch 577, without it 574)
-        if (far) {
+        if (__builtin_expect(far, 0)) {
             const float own = is_far(mx) ? mx : 0.f;
 #pragma unroll
             for (int n = 0; n < NS; ++n)
@@ -468,46 +469,67 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
             plain_step(k_even, v_even, k_odd, v_odd, std::false_type{});
             plain_step(k_odd, v_odd, k_even, v_even, std::true_type{});
         }
-        const int odd_from = k0;                                         // first key of the masked steps
+        odd_from = k0;                                                   // first key of the masked steps
         while (it < steps) {
             masked_step(k_even, v_even, k_odd, v_odd);
             if (it >= steps) break;
             masked_step(k_odd, v_odd, k_even, v_even);
         }
-
-        // (rare) NaNs and infinities in V rows of masked steps reach the rows that see them: a weight of any size times such a
-        // value is that value.
-        if (__builtin_amdgcn_readfirstlane(s_odd)) {
-#pragma unroll 1
-            for (int key = odd_from; key < k_end; ++key) {
-                const int page = __builtin_amdgcn_readfirstlane(page_of(a.cache, table, key));
-                if (page < 0) continue;
-                const T* v = static_cast<const T*>(a.v_pages) + paged_offset(a.cache, page, kvh, key);
-                const __amdgpu_buffer_rsrc_t w = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(v), 0, D * (int)sizeof(T), 0x00020000);
-                const bool see = key <= limit;
-                int at = 4 * half * (int)sizeof(T);
-                asm volatile("" : "+v"(at));                   // (offsets made here, not held in registers across the steps)
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int r4 = 0; r4 < 4; ++r4) {
-                        const Quad<T> x = load_quad<T>(w, at + (32 * d + 8 * r4) * (int)sizeof(T));
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float f = to_f32(x.v[e]);
-                            o[d][4 * r4 + e] += see && !(__builtin_fabsf(f) < INFINITY) ? f : 0.f;
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-            }
-        }
     }
 
     l += __shfl_xor(l, 32, kWave);
+    // (rare) NaNs and infinities in V.  A weight of any size times such a value is that value - also one that has become zero in the type, whose
+    // product with it is NaN - so a component of a row is the sum of those that it sees in the component's column, if there are any.
+    // Masked steps left them out (s_odd); plain steps show them by a sum that is not finite although the weights' is.
+    bool anywhere = false;
+    if (odd_from > k_begin) {
+        f32x4 probe = {0.f, 0.f, 0.f, 0.f};                    // (sums of zeros or NaNs)
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) probe[r % 4] = __builtin_fmaf(o[d][r], 0.f, probe[r % 4]);
+        anywhere = __builtin_amdgcn_ballot_w64((probe[0] + probe[1]) + (probe[2] + probe[3]) != 0.f && l < INFINITY) != 0;
+    }
+    if (__builtin_expect(k_begin < k_end && (anywhere || __builtin_amdgcn_readfirstlane(s_odd)), 0)) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            f32x16 sum;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum[r] = 0.f;
+#pragma unroll 1
+            for (int row0 = anywhere ? k_begin : odd_from; row0 < k_end; row0 += kRowGroup) {
+                const int page = __builtin_amdgcn_readfirstlane(page_of(a.cache, table, row0));
+                if (page < 0) continue;
+                const T* v = static_cast<const T*>(a.v_pages) + paged_offset(a.cache, page, kvh, row0);
+                const __amdgpu_buffer_rsrc_t w = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(v), 0, rows_left(k_end, row0) * D * (int)sizeof(T), 0x00020000);
+#pragma unroll 1
+                for (int r0 = 0; r0 < kRowGroup; r0 += 4) {           // four rows' loads in flight
+                    Quad<T> x[4][4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int r4 = 0; r4 < 4; ++r4) {
+                            const int c = 32 * d + 8 * r4 + 4 * half;
+                            x[i][r4] = load_quad<T>(w, c < D ? ((r0 + i) * D + c) * (int)sizeof(T) : (int)kOutside);
+                        }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const float f = to_f32(x[i][r / 4].v[r % 4]);
+                            sum[r] += row0 + r0 + i <= limit && !(__builtin_fabsf(f) < INFINITY) ? f : 0.f;
+                        }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = __builtin_fabsf(sum[r]) < INFINITY ? o[d][r] : sum[r];
+        }
+    }
+
     // (rare) No sum although there are rows up to the limit: either none of them has a page, or all scores are -inf, and then there is no
     // distribution - NaN, unless another piece has one: its maximum is above the lowest value that stands here for "saw only -inf".
     bool lost = false;
-    if (__builtin_amdgcn_ballot_w64(l == 0.f && limit >= k_begin) != 0) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(l == 0.f && limit >= k_begin) != 0, 0)) {
 #pragma unroll 1
         for (int row = k_begin; row < k_end; row += kRowGroup) {
             const int page = __builtin_amdgcn_readfirstlane(page_of(a.cache, table, row));
@@ -594,7 +616,7 @@ void paged_prompt_merge_kernel(const PromptArgs a)
     if ((int)threadIdx.x >= per * nq || row >= rows) return;
     const int token = row / a.Hq, head = row % a.Hq;
     float M = -INFINITY, L = 0.f;
-    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    f32x4 O = {0.f, 0.f, 0.f, 0.f}, odd = O;               // (odd: NaNs and infinities, which no weight changes)
     for (int s0 = 0; s0 < a.nsplit; s0 += BATCH) {
         float m[BATCH], l[BATCH];
         f32x4 x[BATCH];
@@ -620,7 +642,11 @@ void paged_prompt_merge_kernel(const PromptArgs a)
             const float w = on ? __builtin_amdgcn_exp2f((m[j] - bm) * a.score_scale) : 0.f;
             L = on ? __builtin_fmaf(l[j], w, L) : L;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) O[e] = on ? __builtin_fmaf(x[j][e], w, O[e]) : O[e];
+            for (int e = 0; e < 4; ++e) {
+                const bool finite = __builtin_fabsf(x[j][e]) < INFINITY;
+                O[e] = on && finite ? __builtin_fmaf(x[j][e], w, O[e]) : O[e];
+                odd[e] += on && !finite ? x[j][e] : 0.f;
+            }
         }
         M = bm;
     }
@@ -634,7 +660,7 @@ void paged_prompt_merge_kernel(const PromptArgs a)
     const float inv = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;          // (no piece saw a row: zeros; only scores of -inf: 0 / 0)
     T* out = static_cast<T*>(a.out) + (size_t)token * a.out_stride + (size_t)head * a.cache.D + c;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = from_f32<T>(O[e] * inv);
+    for (int e = 0; e < 4; ++e) out[e] = from_f32<T>((__builtin_fabsf(odd[e]) < INFINITY ? O[e] : odd[e]) * inv);
 }
 
 template <typename T>
