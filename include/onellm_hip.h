@@ -344,7 +344,8 @@ size_t onellm_paged_prompt_attn_workspace_bytes(int B, int token_num, int Hq, in
  *   workspace, workspace_bytes  onellm_paged_decode_attn_workspace_bytes(), 256-byte aligned; calls of different shapes may
  *         share one (a zero-filled one too), calls that overlap in time may not
  * History rows without a page take no part; the new token's own row always does, and is stored where it has a page.  The
- * new rows are rounded to the cache's type before they take part; all arithmetic is fp32 or better.  The result does not
+ * new rows are rounded to the cache's type before they take part; all arithmetic is fp32 or better.  NaNs and infinities as in
+ * onellm_paged_prompt_attn.  The result does not
  * depend on the order in which workgroups finish.
  */
 int onellm_paged_decode_attn(int dtype, const void* qkv, const void* qkv_bias, void* k_pages, void* v_pages, void* out,

@@ -105,6 +105,27 @@ __device__ __forceinline__ f32x4 join_waves(const float* st_ml, const float* acc
 // two neighbouring columns of a row
 template <typename T> struct alignas(2 * sizeof(T)) Pair { T a, b; };
 
+__device__ __forceinline__ bool all_finite(f32x4 v)
+{
+    return __builtin_fabsf(v[0]) + __builtin_fabsf(v[1]) + __builtin_fabsf(v[2]) + __builtin_fabsf(v[3]) < INFINITY;
+}
+__device__ __forceinline__ float odd_part(float v) { return __builtin_fabsf(v) < INFINITY ? 0.f : v; }     // of NaNs and infinities
+
+// four neighbouring columns out of a window
+template <typename T>
+__device__ __forceinline__ f32x4 load_quad(__amdgpu_buffer_rsrc_t w, unsigned offset)
+{
+    f32x4 v;
+    if constexpr (sizeof(T) == 2) {
+        const f16x4 x = __builtin_bit_cast(f16x4, __builtin_amdgcn_raw_buffer_load_b64(w, offset, 0, 0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)x[e];
+    } else {
+        v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(w, offset, 0, 0));
+    }
+    return v;
+}
+
 template <typename T>
 __device__ __forceinline__ void store_quad(T* out, f32x4 v)
 {
@@ -401,11 +422,37 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
     __syncthreads();
     const int nq = D / 4;                                     // quads of a head
     T* out = static_cast<T*>(p.out) + ((size_t)u.b * a.Hq + u.kvh * a.G + u.g0) * D;
+    // (rare) NaNs and infinities in V: a component is the sum of those in its column, whatever their weights.  A weight that is zero in the type, or
+    // the remainder of one, makes NaN of an infinity; so where a sum is not finite although the weights' is, the piece's rows are looked
+    // through for such values.  (Here and not on the waves' sums: there it waited for the rows requested behind the last step, 0.4 us)
+    auto odd_values = [&](f32x4 O, float L, int c) __attribute__((always_inline)) {
+        if (__builtin_expect(!all_finite(O) && L < INFINITY, 0)) {
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int row0 = u.r0; row0 < r1; row0 += kRowGroup) {
+                const int page = __builtin_amdgcn_readfirstlane(page_of(p.cache, table, row0));
+                const __amdgpu_buffer_rsrc_t w = row_window(p.v_pages, page, row0);
+#pragma unroll
+                for (int r = 0; r < kRowGroup; ++r) {
+                    const f32x4 x = load_quad<T>(w, (unsigned)((r * D + c) * (int)sizeof(T)));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[e] += odd_part(x[e]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (u.is_last) sum[e] += odd_part(sv[c + e]);
+                O[e] = __builtin_fabsf(sum[e]) < INFINITY ? O[e] : sum[e];
+            }
+        }
+        return O;
+    };
     if (u.direct) {
         for (int i = tid; i < ng * nq; i += kThr) {
             const int g = i / nq, c = (i % nq) * 4;
             float M, L;
             f32x4 O = join_waves<S, DP>(st_ml, scratch, snew, sv, u.is_last, g, c, M, L);
+            O = odd_values(O, L, c);
             const float inv = 1.f / L;                        // (the new token's row is always there)
 #pragma unroll
             for (int e = 0; e < 4; ++e) O[e] *= inv;
@@ -426,7 +473,8 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
     for (int i = tid; i < ng * nq; i += kThr) {
         const int g = i / nq, c = (i % nq) * 4;
         float M, L;
-        const f32x4 O = join_waves<S, DP>(st_ml, scratch, snew, sv, u.is_last, g, c, M, L);
+        f32x4 O = join_waves<S, DP>(st_ml, scratch, snew, sv, u.is_last, g, c, M, L);
+        O = odd_values(O, L, c);
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, O), wo, (entry(wg, g) * D + c) * 4u, 0, kDevice);
         if (c == 0) {
             typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
@@ -492,6 +540,22 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
 #pragma unroll
                 for (int e = 0; e < 4; ++e) O[e] = s0 + j < P ? __builtin_fmaf(y[e], f, O[e]) : O[e];
             }
+        }
+        if (__builtin_expect(!all_finite(O), 0)) {            // (rare) the pieces' NaNs and infinities are not weighted
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int s0 = first * BATCH; s0 < P; s0 += slices * BATCH) {
+                fetch(s0);
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) {
+                    const float f = wgt[min(s0 + j, P - 1) * ng + g];
+                    const f32x4 y = __builtin_bit_cast(f32x4, x[j]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[e] += s0 + j < P ? __builtin_fmaf(f, 0.f, odd_part(y[e])) : 0.f;       // (a NaN weight wins)
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[e] = __builtin_fabsf(sum[e]) < INFINITY ? O[e] : sum[e];
         }
         if (slices > 1) {
             if (on) part[slice * quads + quad] = O;
