@@ -249,7 +249,11 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs& p, const RopeTurn
         for (int j = 0; j < 2; ++j) {
             if (i0 + j * kThr >= rows_new * half_d) continue;
             const int g = ng_[j], pr = npair[j];
-            float x0 = to_f32(nx[j].a) + (bias ? to_f32(ny[j].a) : 0.f), x1 = to_f32(nx[j].b) + (bias ? to_f32(ny[j].b) : 0.f);
+            float x0 = to_f32(nx[j].a), x1 = to_f32(nx[j].b);
+            if (bias) {                                       // (adding zero would turn -0 into +0, which the store does not)
+                x0 += to_f32(ny[j].a);
+                x1 += to_f32(ny[j].b);
+            }
             if (g <= ng && 2 * pr < a.rotary_dim) {
                 float sn, cs;
                 rope_sincos(pos, rt.f[pr], sn, cs);
