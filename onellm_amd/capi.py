@@ -278,7 +278,7 @@ def _rows(t, what, here):
     """(pointer, token stride) of a [tokens, heads, D] tensor whose tokens may be a stride apart"""
     tokens, heads, d = t.shape
     s0, s1, s2 = t.stride()
-    if s2 != 1 or s1 != d:
+    if s2 != 1 or (s1 != d and heads > 1):
         raise ValueError(f"{what}: [tokens, heads, D] with contiguous heads expected")
     if t.get_device() != here:
         raise ValueError(f"{what}: tensor on {t.device}, not on the current device")
