@@ -3,7 +3,7 @@
 //   lse = log sum_v exp(x_v);   logprob = x_target - lse;   entropy = lse - sum_v p_v x_v,  p_v = exp(x_v - lse)
 //
 // One pass: N * V * e bytes read once.  Sums are taken in units of log 2 against a running maximum per thread and joined at
-// the end; with y = (x - reference) * log2(e):  Z = sum 2^y,  S = sum 2^y y,  logprob = ln 2 (y_target - log2 Z),
+// the end; with y = (x - reference) * log2(e):  Z = sum 2^y,  S = sum 2^y y,  logprob = (x_target - reference) - ln 2 log2 Z,
 // entropy = ln 2 (log2 Z - S / Z) - differences only, so a row of large or very negative logits loses nothing.
 // Per logit that is a multiply-add, an exponential (two issue slots), an add and for the entropy a clamp and a multiply-add; with
 // half a slot for the maximum that is 6.5 slots, 22 us for 4096 x 32000 logits on all SIMDs against 37 us to read them in fp16.
@@ -66,11 +66,17 @@ template <typename T> __device__ __forceinline__ float exponent(float x, float r
 {
     return sizeof(T) == 2 ? __builtin_fmaf(x, kLog2e, -ref) : (x - ref) * kLog2e;
 }
-// the log-probability of logit x, log2 Z = logz
-template <typename T> __device__ __forceinline__ float logprob_of(float x, float ref, float logz)
+// What a row's results are made of: its largest logit and log2 of the sum against that.  Of an fp16 row the logit comes back out of the
+// reference (its product with log2(e), rounded once: the nearest fp16 value is the logit), and the reference's rounding, which the
+// sums carry, is taken off; so a log-probability is a difference of logits and a small logarithm, rounded once, in both types.
+struct RowSum { float max, logz; };
+template <typename T> __device__ __forceinline__ RowSum row_sum(float ref, float logz)
 {
-    return sizeof(T) == 2 ? (exponent<T>(x, ref) - logz) * kLn2 : (x - ref) - logz * kLn2;
+    if constexpr (sizeof(T) == 4) return {ref, logz};
+    const float max = (float)(_Float16)(ref * kLn2);
+    return {max, logz - __builtin_fmaf(max, kLog2e, -ref)};
 }
+__device__ __forceinline__ float logprob_of(float x, RowSum r) { return (x - r.max) - r.logz * kLn2; }
 template <typename T> __device__ __forceinline__ float exponent_between(float ref, float to)      // of one reference against another
 {
     return sizeof(T) == 2 ? ref - to : (ref - to) * kLog2e;
@@ -179,12 +185,13 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int row, Stats s
 {
     const T* x = static_cast<const T*>(a.logits) + (size_t)row * a.ld;
     const float logz = __builtin_amdgcn_logf(st.z);           // log2
+    const RowSum sum = row_sum<T>(st.ref, logz);
     const bool empty = st.ref == -INFINITY && st.z == 0.f;    // no logit above -inf (and no NaN): no distribution
     if (lane == 0) {
         if (a.logprob) {
             const int t = a.targets[row];
             float v = 0.f;
-            if ((unsigned)t < (unsigned)a.V) v = empty ? -INFINITY : logprob_of<T>(to_f32(x[t]), st.ref, logz);
+            if ((unsigned)t < (unsigned)a.V) v = empty ? -INFINITY : logprob_of(to_f32(x[t]), sum);
             a.logprob[row] = v;
         }
         if (a.entropy) a.entropy[row] = empty ? 0.f : (logz - st.s / st.z) * kLn2;
@@ -194,7 +201,7 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int row, Stats s
         float v = -INFINITY;
         if (i < ntop) {
             id = id_of(top[i]);
-            v = logprob_of<T>(value_of((unsigned)(top[i] >> 32)), st.ref, logz);
+            v = logprob_of(value_of((unsigned)(top[i] >> 32)), sum);
         }
         a.top_ids[(size_t)row * a.K + i] = id;
         a.top_logprobs[(size_t)row * a.K + i] = v;
