@@ -318,7 +318,9 @@ int onellm_paged_qkv_store(int dtype, void* q_out, long q_stride, void* k_pages,
  * token_num * (Hq / Hkv) / 128 + min(B, token_num) <= 65535 (two million tokens of four heads per kv head): else ONELLM_EUNSUPPORTED.
  *   max_rows   upper bound of every sequence's history + tokens; where few tokens meet many rows it sizes the cut of the
  *              rows into pieces (a longer sequence is still attended in full, slower; a bound far above the longest one cuts
- *              what need not be cut, some 10 us)
+ *              what need not be cut, some 10 us).  An fp16 call of more than 384 workgroups - kv heads times tiles of 128 rows of
+ *              tokens * (Hq / Hkv), one more per sequence - is not cut: a few tokens behind 20000 rows are better off in a call of
+ *              their own than beside dozens of short prompts (37 + 20 us against 392)
  *   workspace  onellm_paged_prompt_attn_workspace_bytes() bytes, 256-byte aligned, contents irrelevant; calls that share one
  *              must not overlap.  Fewer tokens may need more of it; 786432 (D + 2) + 256 bytes are enough for any call
  * Scores, statistics and sums are fp32; fp16 weights enter their product rounded to fp16.

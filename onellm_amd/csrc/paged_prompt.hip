@@ -685,15 +685,20 @@ long tiles_bound(int B, int token_num, int G)
 }
 
 // Pieces the rows of the cache are cut into.  fp16, 256 workgroups or fewer: the longest tile takes 20 ns per row and 128 columns, so n
-// pieces a 1 / n of that (1.45 / n where two share a compute unit); they cost a second launch, 4 us, and each the states' way through
-// memory twice, at 6 TB/s.  The n that is best so, up to two workgroups per compute unit and 128 rows per piece.
+// pieces a 1 / n of that (1.45 / n where two share a compute unit, 2 / n with heads above 128, where the second one waits for the
+// first); they cost a second launch, 4 us, and each the states' way through memory twice, at 6 TB/s.  The n that is best so, up to two
+// workgroups per compute unit and 128 rows per piece.  Heads of 256, 1.45 / 2: 5 tokens of 32 heads on 8 behind 20000 rows 63.0 / 47.9 us, 1000 of
+// 8 on 2 behind 3000 76.7 / 63.1, 461 of 16 on 4 behind 15000..20000 247.7 / 246.6; of 160: 61.6 / 46.6, 71.4 / 59.6, 214 / 214.
 // 461 tokens behind 15000..20000 rows (120 workgroups) 1 / 2 / 3 / 4 / 5 pieces 404 / 230 / 217 / 185 / 224 us (four), 512 tokens of 32 heads
 // on 8 uncut / two 18.1 / 22.3 (uncut), 64 behind 800 uncut / three / six 24.2 / 18.4 / 16.1 (six), 1000 of 8 heads on 2 uncut / three
 // 26.4 / 21.1 (three), 1000 of 32 on 8 behind 3000 uncut / two 92.5 / 83.8 (two), 400 behind 1000 two / five 29.5 / 33.1 (two).
 // A little more than one workgroup per compute unit, fp16: the longest end long after the others, so two pieces if the tiles' rows
-// differ much, as those of several sequences and of one with little before it do, and are many.  Uncut / two pieces: 4096 tokens of 8
-// heads on one (257 workgroups) 88 / 68 us, 6000 (376) 135 / 107, 500 + 500 + 200 tokens behind 500..3000 rows (320) 77 / 64, 8 x 150 behind
-// 100..3000 (360) 77 / 65; but 1400 tokens (352) 40 / 51, 1100 behind 1000 rows (280) 53 / 65, 1600 behind 6000 (408) 210 / 227.
+// differ much and are many, as those of one sequence with little before it do, and those of several sequences may - only the device knows
+// their lengths, and unequal ones gain more than equal ones lose.  Uncut / two pieces: 4096 tokens of 8
+// heads on one (257 workgroups) 88 / 68 us, 6000 (376) 135 / 107, 500 + 500 + 200 tokens behind 500..3000 rows (320) 70 / 59, 8 x 150 behind
+// 100..3000 (360) 70 / 60, 4 x 330 behind 6000 each 183 / 177, but 8 x 160 behind 3000 each (384) 96 / 103, 2 x 700 behind 2000 80 / 86; 1400
+// tokens (352) 40 / 51, 1100 behind 1000 rows (280) 53 / 65, 1600 behind 6000 (408) 210 / 227.  More workgroups than that are not cut,
+// however long one tile is: 5 tokens behind 20000 rows beside 40 prompts of 60 tokens 392 us, in a call of their own 37 and the prompts 20.
 // fp32: a tile's steps take six times as long, so the longest tile of a call ends long after the others unless it is cut: three
 // workgroups per compute unit (two where heads of more than 128 leave room for one at a time), pieces of 128 rows or more.
 // Pieces 1 / 2 / 3 / 4 / 8: 2058 tokens in 4 sequences (264 workgroups) 100 / 85 / 63 / 74 / 87 us, 2048 tokens (520) 384 / 328 / 322 / 345 / 430,
@@ -713,7 +718,7 @@ int split_of(int dtype, int B, int token_num, long tiles, int Hq, int Hkv, int D
         double best = whole;
         n = 1;
         for (int two = 0; two < 2; ++two) {
-            const double sole = two ? 1.45 * whole : whole;
+            const double sole = two ? (D <= 128 ? 1.45 : 2.0) * whole : whole;
             long c = two ? (512 + wgs / 2) / wgs : 256 / wgs;
             if (c > most) c = most;
             if (c * c * piece > sole) c = (long)(sqrt(sole / piece) + 0.5);
