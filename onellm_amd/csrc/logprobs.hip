@@ -6,8 +6,10 @@
 // the end; with y = (x - reference) * log2(e):  Z = sum 2^y,  S = sum 2^y y,  logprob = (x_target - reference) - ln 2 log2 Z,
 // entropy = ln 2 (log2 Z - S / Z) - differences only, so a row of large or very negative logits loses nothing.
 // Per logit that is a multiply-add, an exponential (two issue slots), an add and for the entropy a clamp and a multiply-add; with
-// half a slot for the maximum that is 6.5 slots, 22 us for 4096 x 32000 logits on all SIMDs against 37 us to read them in fp16.
-// Measured: 55 us with entropy and the 8 best (47..50 without the list), 4.8 TB/s; 16 x 32000 fp32 and the 5 best 9.5 us, two launches.
+// half a slot for the maximum that is 6.5 slots, 22 us for 4096 x 32000 logits on all SIMDs against 37 us to read them in fp16.  Counted
+// are 12.6 slots, 41 us: as much again as the logits' own goes into each row's tail (floor, candidates, joins of 256 lanes), with
+// nothing of the next row on its way.
+// Measured: 54 us with entropy and the 8 best (46 without the list), 4.8 TB/s; 16 x 32000 fp32 and the 5 best 9.5 us, two launches.
 //
 // The K best: a wave keeps candidates in LDS as 64-bit keys (value, then lower token first).  The K-th largest of the first step's
 // 256 lane maxima, found bit by bit with ballots, is a floor below which nothing can be among the K best; the lanes that reach
@@ -424,8 +426,10 @@ void token_logprobs_join_kernel(const LogprobArgs a)
     write_row<T>(a, row, st, list, n, lane);
 }
 
-// Parts per row: one while the rows alone give every compute unit two workgroups, else enough for that, of a step or more each
-// (16 x 32000 fp16, K = 8: two parts of two steps 16.1 us, four of one 12.1; 64 x 128000: 20.4, 15.3).
+// Parts per row: one where the rows alone give every compute unit two workgroups, else as many as that takes, but at most kMaxParts and
+// one per step (16384 logits in fp16, 8192 in fp32), so few rows do not fill the chip.  Whole / in parts: 16 x 32000 fp16, K = 8 (two parts)
+// 12.0 / 11.7 us, fp32, K = 5 (four) 13.6 / 11.1; 64 x 128000 fp16 (eight) 30.3 / 14.9; one row of 150000 (ten) 26.1 / 16.9; 300 x 32000 (two)
+// 14.4 / 15.3.
 int parts_of(int N, int V, int step)
 {
     int n = N >= 512 ? 1 : (511 + N) / N;

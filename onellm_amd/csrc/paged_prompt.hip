@@ -15,9 +15,10 @@
 //
 // 128 rows per workgroup: every K and V row that comes through LDS is then used for 128 products, and a wave's 32 rows of scores, output
 // and Q leave room for two workgroups on a compute unit (heads up to 128), of which one multiplies while the other takes exponentials.
-// Bound by that pair of units, not by memory: 8192 tokens of 32 heads on 8 of 128, fp16, 550 us, 1000 TFLOP/s (a library product of
-// 16384^3 reaches 1266 on the same card), matrix cores 54 % busy and the vector unit 50 %.  2058 tokens in four sequences, fp32, 16 heads on 2
-// of 64: 62 us.
+// Bound by that pair of units, not by memory: 8192 tokens of 32 heads on 8 of 128, fp16, 544..577 us, 950..1010 TFLOP/s (a library product
+// of 16384^3 reaches 1266 on the same card), matrix cores 54 % busy and the vector unit 53 %.  2058 tokens in four sequences, fp32, 16 heads on 2
+// of 64: 62.5 us.  Heads between 64, 128 and 256 are multiplied at the next of these: 8192 tokens with heads of 96 / 160 / 192 / 256 506 / 1436 /
+// 1446 / 1464 us.
 #include <type_traits>
 #include "paged.hpp"
 
