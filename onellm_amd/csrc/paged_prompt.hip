@@ -531,10 +531,11 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a)
     // distribution - NaN, unless another piece has one: its maximum is above the lowest value that stands here for "saw only -inf".
     bool lost = false;
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(l == 0.f && limit >= k_begin) != 0, 0)) {
-#pragma unroll 1
-        for (int row = k_begin; row < k_end; row += kRowGroup) {
-            const int page = __builtin_amdgcn_readfirstlane(page_of(a.cache, table, row));
-            lost = lost || (page >= 0 && row <= limit && l == 0.f);
+        for (int block = 0; k_begin + block * kWave * kRowGroup < k_end; ++block) {
+            const unsigned long long has = __builtin_amdgcn_ballot_w64(pages_of(block) >= 0);
+            const int upto = (limit - k_begin) / kRowGroup - block * kWave;       // the last group of the block that the row sees
+            const unsigned long long seen = upto < 0 ? 0 : upto < kWave - 1 ? (2ull << upto) - 1 : ~0ull;
+            lost = lost || (l == 0.f && limit >= k_begin && (has & seen) != 0);
         }
         if (lost) mx = kLowest;
     }

@@ -65,3 +65,23 @@ def test_decode(capi, dev, dtype):
     c.qkv[1:, 4:6, 5] = -math.inf                             # the new token's key too
     got = decode(capi, c)
     assert torch.isnan(got[1:]).all() and torch.equal(got[0], clean[0])
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("cut", [False, True])
+def test_prompt_behind_rows_that_have_no_page(capi, dev, dtype, cut):
+    """The first tokens see only pages that are none, the next ones one page of scores of -inf, the last ones another key as well"""
+    c = pm.Case(dtype, [100], [2200], 2, 1, 64, 16, seed=67)
+    c.q[:, :, 5] = 1.0
+    c.table[0, :140] = -1                                     # rows 0 .. 2239: tokens 0 .. 39 see nothing
+    for r in range(2240, 2256):
+        row(c, c.kp, 0, r)[0, 5] = -math.inf
+    top = c.max_rows if cut else 1
+    assert is_cut(capi, c, top) == cut
+    got = prompt(capi, c, top)
+    assert (got[:40] == 0).all()
+    assert torch.isnan(got[40:56]).all()
+    assert torch.isfinite(got[56:]).all()
+    c.table[0, 140] = -1
+    clean = prompt(capi, c, top)
+    assert (clean[:56] == 0).all() and torch.equal(clean[56:], got[56:])
