@@ -11,7 +11,8 @@
 // the keys its lanes hold, and V^T's operand picks the same keys.  For fp16 that operand (a column of V over four
 // keys) comes out of the LDS transposed (ds_read_b64_tr_b16); for fp32 a product takes two keys and reads them as they are.
 // Scores, statistics and output are fp32.  fp16: P enters its product rounded to fp16 (half a step, 2^-11 relative of each
-// weight, averaged over the keys); the sum of the weights is taken before that rounding.
+// weight, averaged over the keys: together at most about what the result's own rounding adds); the sum of the weights is taken before
+// that rounding.  P in two parts, 8192 tokens: 781 us instead of 574.
 //
 // 128 rows per workgroup: every K and V row that comes through LDS is then used for 128 products, and a wave's 32 rows of scores, output
 // and Q leave room for two workgroups on a compute unit (heads up to 128), of which one multiplies while the other takes exponentials.
